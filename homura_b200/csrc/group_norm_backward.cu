@@ -1,0 +1,373 @@
+// Group norm with an activation, channels last, the gradients (include/homura_cuda_layers.h); tiles as in group_norm.cuh.
+//
+// Three steps: sums over each run of rows of dz and dz * xhat (by channel for weight and bias, by group, weighted, for
+// the input), a small kernel that folds the runs in order, and an elementwise pass. Channel sums are kept in f64 across
+// the runs a block takes, and folded over the blocks in f64.
+#include "group_norm.cuh"
+
+namespace hmc {
+namespace gnorm {
+namespace {
+
+struct GradArgs {
+    char *dsrc, *dweight, *dbias;  // dweight, dbias: or null
+    const char *src, *dout, *mean, *rstd;
+    Rows wdsrc, wsrc, wdout;
+    int64_t mean_n, mean_g, rstd_n, rstd_g, dweight_stride, dbias_stride;
+    int32_t dparam_f32;
+    Tiling t;
+    Cut cut;              // of the sums
+    int64_t columns;      // blocks that share a tile of channels
+    Cut apply;
+    int64_t positions, samples;
+    Affine affine;
+    void *pieces;         // Two<C> [samples][groups][chunks * segments]
+    void *means;          // Two<C> [samples][groups]: the means of p and of p * xhat
+    double *by_channel;   // [columns][2][channels], null when neither dweight nor dbias is wanted
+};
+
+// One element: xhat and dz, with the forward pass's steps (unfused) up to z.
+template <class T, int ACT, class C>
+__device__ __forceinline__ void element(C x, C dy, C mean, C rstd, C w, C b, C &xhat, C &dz) {
+    xhat = (x - mean) * rstd;
+    const C z = xhat * w + b;
+    dz = through<ACT, C, sizeof(T) == 2>(dy, z);
+}
+
+template <class T, int V> struct Coefficients {
+    typename Comp<T>::C mean[V], rstd[V], w[V], b[V];
+    __device__ __forceinline__ void load(const GradArgs &a, int64_t sample, const Tile &tile, int at) {
+        using C = typename Comp<T>::C;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int64_t group = tile.group + (at + i) / tile.part;
+            mean[i] = reinterpret_cast<const C *>(a.mean)[sample * a.mean_n + group * a.mean_g];
+            rstd[i] = reinterpret_cast<const C *>(a.rstd)[sample * a.rstd_n + group * a.rstd_g];
+        }
+    }
+    __device__ __forceinline__ void load_affine(const GradArgs &a, int64_t channel) {
+        using C = typename Comp<T>::C;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            w[i] = a.affine.weight != nullptr ? parameter<T>(a.affine.weight, (channel + i) * a.affine.weight_stride, a.affine.is_f32) : C(1);
+            b[i] = a.affine.weight != nullptr ? parameter<T>(a.affine.bias, (channel + i) * a.affine.bias_stride, a.affine.is_f32) : C(0);
+        }
+    }
+};
+
+// Block b of tile t takes the (sample, chunk) pairs b, b + columns, ... in order.
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kBlock, 2) sums_kernel(const __grid_constant__ GradArgs a) {
+    using C = typename Comp<T>::C;
+    __shared__ union {
+        C by_row[2][kBlock * V];
+        double by_column[kBlock * V];
+    } shared;
+    __shared__ C first[kBlock * V];
+    const int tx = threadIdx.x % a.t.tx, ty = threadIdx.x / a.t.tx;
+    const int64_t index = blockIdx.x / a.columns, column = blockIdx.x - index * a.columns;
+    const Tile tile = tile_at(a.t, index);
+    const bool live = tx * V < tile.width && ty < a.t.ty;
+    const int64_t channel = tile.channel + tx * V;
+    Coefficients<T, V> k;
+    if (live) k.load_affine(a, channel);
+    double dw[V], db[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) dw[i] = db[i] = 0.0;
+    const int64_t pairs = a.samples * a.cut.chunks;
+    const int64_t pieces = a.cut.chunks * a.t.segments;
+    for (int64_t pair = column; pair < pairs; pair += a.columns) {
+        const int64_t sample = pair / a.cut.chunks, chunk = pair - sample * a.cut.chunks;
+        const int64_t begin = chunk * a.cut.run;
+        const int64_t end = begin + a.cut.run < a.positions ? begin + a.cut.run : a.positions;
+        C s1[V], s2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) s1[i] = s2[i] = C(0);
+        if (live) {
+            k.load(a, sample, tile, tx * V);
+            const T *src = reinterpret_cast<const T *>(a.src) + sample * a.wsrc.n + channel;
+            const T *dout = reinterpret_cast<const T *>(a.dout) + sample * a.wdout.n + channel;
+#pragma unroll 4
+            for (int64_t row = begin + ty; row < end; row += a.t.ty) {
+                const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(src + row * a.wsrc.s);
+                const Pack<T, V> d = *reinterpret_cast<const Pack<T, V> *>(dout + row * a.wdout.s);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    C xhat, dz;
+                    element<T, ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
+                    s1[i] += dz;
+                    s2[i] = m_fma(dz, xhat, s2[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                db[i] += static_cast<double>(s1[i]);
+                dw[i] += static_cast<double>(s2[i]);
+                shared.by_row[0][ty * tile.width + tx * V + i] = s1[i] * k.w[i];
+                shared.by_row[1][ty * tile.width + tx * V + i] = s2[i] * k.w[i];
+            }
+        }
+        __syncthreads();
+        Two<C> *to = reinterpret_cast<Two<C> *>(pieces == 1 ? a.means : a.pieces) + (sample * a.t.groups + tile.group) * pieces + chunk * a.t.segments + tile.segment;
+        const C scale = pieces == 1 ? C(1) / (static_cast<C>(a.positions) * static_cast<C>(a.t.cg)) : C(1);
+        by_group(shared.by_row[0], tile, a.t.ty, [&](int q, C s) { first[q] = s; });
+        __syncthreads();
+        by_group(shared.by_row[1], tile, a.t.ty, [&](int q, C s) { to[q * pieces] = Two<C>{first[q] * scale, s * scale}; });
+        __syncthreads();
+    }
+    if (a.by_channel == nullptr) return;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) shared.by_column[ty * tile.width + tx * V + i] = which == 0 ? dw[i] : db[i];
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < tile.width; c += kBlock) {
+            double sum = 0.0;
+            for (int y = 0; y < a.t.ty; ++y) sum += shared.by_column[y * tile.width + c];
+            a.by_channel[(column * 2 + which) * a.t.channels + tile.channel + c] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// A warp folds the pieces of a group: every lane its own in order, then the lanes in a fixed tree.
+template <class C> __global__ void __launch_bounds__(kBlock) fold_groups_kernel(const __grid_constant__ GradArgs a, int64_t total) {
+    const int lane = threadIdx.x & 31;
+    const int64_t pieces = a.cut.chunks * a.t.segments;
+    const double count = static_cast<double>(a.positions) * static_cast<double>(a.t.cg);
+    for (int64_t g = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); g < total; g += static_cast<int64_t>(gridDim.x) * kWarps) {
+        const Two<C> *p = reinterpret_cast<const Two<C> *>(a.pieces) + g * pieces;
+        double s = 0.0, t = 0.0;
+        for (int64_t k = lane; k < pieces; k += 32) {
+            s += static_cast<double>(p[k].a);
+            t += static_cast<double>(p[k].b);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+            t += __shfl_xor_sync(0xFFFFFFFFu, t, d);
+        }
+        if (lane == 0) reinterpret_cast<Two<C> *>(a.means)[g] = Two<C>{static_cast<C>(s / count), static_cast<C>(t / count)};
+    }
+}
+
+// dweight and dbias: 32 channels a block, eight warps along the blocks that hold partial sums.
+template <class T> __global__ void __launch_bounds__(kBlock) fold_channels_kernel(const __grid_constant__ GradArgs a) {
+    __shared__ double part[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int which = static_cast<int>(blockIdx.x & 1);
+    char *to = which == 0 ? a.dweight : a.dbias;
+    if (to == nullptr) return;
+    const int64_t stride = which == 0 ? a.dweight_stride : a.dbias_stride;
+    for (int64_t block = blockIdx.x >> 1; block * 32 < a.t.channels; block += gridDim.x >> 1) {
+        const int64_t channel = block * 32 + lane;
+        double sum = 0.0;
+        if (channel < a.t.channels) {
+            for (int64_t k = warp; k < a.columns; k += kWarps) sum += a.by_channel[(k * 2 + which) * a.t.channels + channel];
+        }
+        part[warp][lane] = sum;
+        __syncthreads();
+        if (warp == 0 && channel < a.t.channels) {
+            for (int w = 1; w < kWarps; ++w) sum += part[w][lane];
+            if (a.dparam_f32) reinterpret_cast<float *>(to)[channel * stride] = static_cast<float>(sum);
+            else reinterpret_cast<T *>(to)[channel * stride] = from_f64<T>(sum);
+        }
+        __syncthreads();
+    }
+}
+
+template <class T, int V, int ACT>
+__global__ void __launch_bounds__(kBlock) grad_kernel(const __grid_constant__ GradArgs a) {
+    using C = typename Comp<T>::C;
+    const int tx = threadIdx.x % a.t.tx, ty = threadIdx.x / a.t.tx;
+    for (int64_t unit = blockIdx.x; unit < a.apply.units; unit += gridDim.x) {
+        const int64_t strip = unit / a.apply.chunks, chunk = unit - strip * a.apply.chunks;
+        const int64_t sample = strip / a.t.tiles;
+        const Tile tile = tile_at(a.t, strip - sample * a.t.tiles);
+        if (tx * V >= tile.width || ty >= a.t.ty) continue;
+        const int64_t channel = tile.channel + tx * V;
+        Coefficients<T, V> k;
+        k.load(a, sample, tile, tx * V);
+        k.load_affine(a, channel);
+        C m1[V], m2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const Two<C> m = reinterpret_cast<const Two<C> *>(a.means)[sample * a.t.groups + tile.group + (tx * V + i) / tile.part];
+            m1[i] = m.a;
+            m2[i] = m.b;
+        }
+        const int64_t begin = chunk * a.apply.run;
+        const int64_t end = begin + a.apply.run < a.positions ? begin + a.apply.run : a.positions;
+        const T *src = reinterpret_cast<const T *>(a.src) + sample * a.wsrc.n + channel;
+        const T *dout = reinterpret_cast<const T *>(a.dout) + sample * a.wdout.n + channel;
+        T *dsrc = reinterpret_cast<T *>(a.dsrc) + sample * a.wdsrc.n + channel;
+#pragma unroll 2
+        for (int64_t row = begin + ty; row < end; row += a.t.ty) {
+            const Pack<T, V> x = *reinterpret_cast<const Pack<T, V> *>(src + row * a.wsrc.s);
+            const Pack<T, V> d = *reinterpret_cast<const Pack<T, V> *>(dout + row * a.wdout.s);
+            Pack<T, V> y;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                C xhat, dz;
+                element<T, ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
+                y.v[i] = down<T>(k.rstd[i] * (dz * k.w[i] - m1[i] - xhat * m2[i]));
+            }
+            *reinterpret_cast<Pack<T, V> *>(dsrc + row * a.wdsrc.s) = y;
+        }
+    }
+}
+
+struct Plan {
+    Tiling t;
+    Cut sums, apply;
+    int64_t columns;
+    int64_t pieces_bytes, means_bytes, bytes;
+};
+Plan make_plan(const Problem &p, bool vectors) {
+    Plan r{};
+    r.t = make_tiling(p.channels, p.groups, 16 / element_size(p.dtype), vectors);
+    r.sums = cut_rows(p, r.t, static_cast<int64_t>(r.t.ty) * 4);
+    r.apply = cut_rows(p, r.t, r.t.ty);
+    const int64_t pairs = p.samples * r.sums.chunks;
+    r.columns = ceil_div(kBlocksWanted, r.t.tiles);
+    if (r.columns > pairs) r.columns = pairs;
+    const int64_t pieces = r.sums.chunks * r.t.segments, es = element_size(p.stat_dtype);
+    r.pieces_bytes = pieces == 1 ? 0 : ceil_div(p.samples * p.groups * pieces * 2 * es, 16) * 16;
+    r.means_bytes = ceil_div(p.samples * p.groups * 2 * es, 16) * 16;
+    r.bytes = r.pieces_bytes + r.means_bytes + r.columns * 2 * p.channels * 8;
+    return r;
+}
+
+}  // namespace
+
+int64_t backward_workspace(const Problem &p) {
+    const int64_t a = make_plan(p, false).bytes;
+    const int64_t b = p.channels % (16 / element_size(p.dtype)) == 0 ? make_plan(p, true).bytes : 0;
+    return a > b ? a : b;
+}
+int64_t forward_workspace(const Problem &p);
+
+}  // namespace gnorm
+}  // namespace hmc
+
+using namespace hmc;
+using namespace hmc::gnorm;
+
+HMC_API hmc_status hmc_group_norm_workspace(const hmc_tensor_desc *src, int32_t groups, int32_t backward, int64_t *bytes) {
+    return guarded([&]() -> hmc_status {
+        if (bytes == nullptr) return fail(HMC_INVALID, "null workspace size");
+        *bytes = 0;
+        hmc_tensor_desc shape{};
+        if (src != nullptr) {  // the size depends on sizes and dtype only: no memory is needed to ask for it
+            shape = *src;
+            static char nothing[16];
+            shape.data = nothing;
+        }
+        Problem p{};
+        hmc_status s = check_problem(src != nullptr ? &shape : nullptr, groups, &p);
+        if (s != HMC_OK) return s;
+        if (p.samples == 0 || p.positions == 0 || p.channels == 0) return HMC_OK;
+        *bytes = backward ? backward_workspace(p) : forward_workspace(p);
+        return HMC_OK;
+    });
+}
+
+HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_desc *dsrc, const hmc_tensor_desc *dweight,
+                                           const hmc_tensor_desc *dbias, const hmc_tensor_desc *src, const hmc_tensor_desc *dout,
+                                           const hmc_tensor_desc *mean, const hmc_tensor_desc *rstd, const hmc_tensor_desc *weight,
+                                           const hmc_tensor_desc *bias, int32_t groups, int32_t activation, void *workspace,
+                                           int64_t workspace_bytes) {
+    return guarded([&]() -> hmc_status {
+        Problem p{};
+        Affine affine{};
+        hmc_status s = check_problem(src, groups, &p);
+        if (s == HMC_OK) s = check_channels_last(src, "the input");
+        if (s == HMC_OK) s = check_layer(dout, "the output's gradient", p.dtype, 3, src->sizes, Use::kInput);
+        if (s == HMC_OK) s = check_channels_last(dout, "the output's gradient");
+        if (s == HMC_OK) s = check_layer(dsrc, "the input's gradient", p.dtype, 3, src->sizes, Use::kOutput);
+        if (s == HMC_OK) s = check_channels_last(dsrc, "the input's gradient");
+        if (s == HMC_OK) s = check_affine(weight, bias, p, &affine);
+        if (s == HMC_OK && (mean == nullptr || rstd == nullptr)) s = fail(HMC_INVALID, "the gradients of group norm need mean and rstd");
+        if (s == HMC_OK) s = check_stats(mean, rstd, p, Use::kInput);
+        if (s == HMC_OK) s = check_activation(activation);
+        int param = -1;
+        for (const hmc_tensor_desc *d : {dweight, dbias}) {
+            if (s != HMC_OK || d == nullptr) continue;
+            if (param < 0) param = weight != nullptr ? weight->dtype : d->dtype;
+            if (weight == nullptr && param != p.dtype && param != HMC_F32) s = fail(HMC_INVALID, "the weight's gradient has neither the input's dtype nor F32");
+            if (s == HMC_OK) s = check_layer(d, d == dweight ? "the weight's gradient" : "the bias's gradient", param, 1, &p.channels, Use::kOutput);
+        }
+        if (s != HMC_OK) return s;
+        const bool empty = p.samples == 0 || p.positions == 0 || p.channels == 0;
+        if (!empty) s = check_workspace(backward_workspace(p), workspace, workspace_bytes);
+        if (s != HMC_OK) return s;
+        HMC_ENTER(ctx);
+        const bool sums_wanted = dweight != nullptr || dbias != nullptr;
+        if (p.channels == 0 || (empty && !sums_wanted)) return HMC_OK;
+        GradArgs a{};
+        a.dsrc = layer_base(dsrc);
+        a.dweight = layer_base(dweight);
+        a.dbias = layer_base(dbias);
+        a.dweight_stride = dweight != nullptr ? dweight->strides[0] : 0;
+        a.dbias_stride = dbias != nullptr ? dbias->strides[0] : 0;
+        a.dparam_f32 = param == HMC_F32 ? 1 : 0;
+        a.samples = p.samples;
+        a.positions = p.positions;
+        const int64_t channel_blocks = 2 * ceil_div(p.channels, 32);
+        if (empty) {  // sums over nothing
+            a.t.channels = p.channels;
+            return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
+                fold_channels_kernel<decltype(tag)><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+                return launch_status("group norm channel kernel launch");
+            });
+        }
+        const Plan plan = make_plan(p, all_vectors(src, dout, dsrc));
+        a.src = layer_base(src);
+        a.dout = layer_base(dout);
+        a.mean = layer_base(mean);
+        a.rstd = layer_base(rstd);
+        a.wdsrc = Rows{dsrc->strides[0], dsrc->strides[1]};
+        a.wsrc = Rows{src->strides[0], src->strides[1]};
+        a.wdout = Rows{dout->strides[0], dout->strides[1]};
+        a.mean_n = mean->strides[0];
+        a.mean_g = mean->strides[1];
+        a.rstd_n = rstd->strides[0];
+        a.rstd_g = rstd->strides[1];
+        a.t = plan.t;
+        a.cut = plan.sums;
+        a.columns = plan.columns;
+        a.apply = plan.apply;
+        a.affine = affine;
+        a.pieces = workspace;
+        a.means = static_cast<char *>(workspace) + plan.pieces_bytes;
+        a.by_channel = sums_wanted ? reinterpret_cast<double *>(static_cast<char *>(a.means) + plan.means_bytes) : nullptr;
+        return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
+            using T = decltype(tag);
+            using C = typename Comp<T>::C;
+            const auto run = [&](auto width) -> hmc_status {
+                constexpr int V = decltype(width)::value;
+                return dispatch_activation(activation, [&](auto act) -> hmc_status {
+                    constexpr int ACT = decltype(act)::value;
+                    sums_kernel<T, V, ACT><<<static_cast<unsigned>(plan.columns * plan.t.tiles), kBlock, 0, ctx->stream>>>(a);
+                    hmc_status l = launch_status("group norm sums kernel launch");
+                    if (l == HMC_OK && plan.sums.chunks * plan.t.segments > 1) {
+                        const int64_t total = p.samples * p.groups;
+                        fold_groups_kernel<C><<<grid_for(ceil_div(total, kWarps)), kBlock, 0, ctx->stream>>>(a, total);
+                        l = launch_status("group norm fold kernel launch");
+                    }
+                    if (l == HMC_OK && sums_wanted) {
+                        fold_channels_kernel<T><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+                        l = launch_status("group norm channel kernel launch");
+                    }
+                    if (l != HMC_OK) return l;
+                    grad_kernel<T, V, ACT><<<grid_for(plan.apply.units), kBlock, 0, ctx->stream>>>(a);
+                    return launch_status("group norm gradient kernel launch");
+                });
+            };
+            if (plan.t.v == kVector<T>) return run(std::integral_constant<int, kVector<T>>{});
+            return run(std::integral_constant<int, 1>{});
+        });
+    });
+}

@@ -16,6 +16,7 @@
 #include "common.cuh"
 #include "elem.cuh"
 #include "map.cuh"
+#include "philox.cuh"
 #include "scan.cuh"
 
 namespace hmc {
@@ -23,32 +24,6 @@ namespace {
 
 constexpr int kSampleThreads = 256;
 constexpr int kBlocksPerThread = 4;  // Philox blocks a thread of the uniform and the unrejected integer sampler takes
-
-struct Words4 {
-    uint32_t w[4];
-};
-
-// Block n under the key [seed, seed >> 32]. src/ops/random.rs:29-51, 75-83.
-__device__ __forceinline__ Words4 philox_block(uint64_t n, uint64_t seed) {
-    constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u;
-    constexpr uint32_t kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
-    uint32_t c0 = static_cast<uint32_t>(n), c1 = static_cast<uint32_t>(n >> 32), c2 = 0, c3 = 0;
-    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
-#pragma unroll
-    for (int round = 0; round < 10; ++round) {
-        if (round > 0) {
-            k0 += kW0;
-            k1 += kW1;
-        }
-        const uint64_t p0 = static_cast<uint64_t>(kM0) * c0;  // one wide multiplication each
-        const uint64_t p1 = static_cast<uint64_t>(kM1) * c2;
-        c0 = static_cast<uint32_t>(p1 >> 32) ^ c1 ^ k0;
-        c1 = static_cast<uint32_t>(p1);
-        c2 = static_cast<uint32_t>(p0 >> 32) ^ c3 ^ k1;
-        c3 = static_cast<uint32_t>(p0);
-    }
-    return Words4{{c0, c1, c2, c3}};
-}
 
 // A uniform f64 in [0, 1) from 53 bits; exact. src/ops/random.rs:86-90.
 __device__ __forceinline__ double unit_f64(uint32_t hi, uint32_t lo) {

@@ -1,0 +1,262 @@
+// What the forward and the backward kernel of the gated linear recurrence share.
+//
+// Both are a scan v_s = c_s v_{s-1} + w_s along one axis for every (batch, channel): forward v = h, c = a, w = u in the
+// order of time; backward v = g, c = the gate of the step processed before, w = dout, against the order of time (rows
+// are addressed in the order they are processed, with negative strides where that runs backwards). The bound is HBM
+// traffic: each element of each operand is moved once.
+//
+// Split. A lane owns V neighbouring channels and, per round, R neighbouring rows that it keeps in registers; a warp is
+// 32 * V channels wide, so a row is one coalesced access. Of a block's eight warps WT divide the time axis among them
+// and 8 / WT the channels; where batch * channels leave SMs idle, up to eight blocks of a cluster divide the time axis
+// further. A round is then R * WT * cluster rows:
+//   1. every lane folds its rows to (A, B): v after the rows = A * (v before) + B;
+//   2. warps leave (A, B) in shared memory, blocks leave their fold in every block's shared memory of the cluster
+//      (distributed shared memory), one barrier each;
+//   3. every lane folds what lies before its rows, always in the order of time, onto the round's carry, and walks its rows
+//      once more from registers, now from the true value, writing the results.
+// No block waits for a block outside its cluster, nothing is read twice, and the order of the folds is fixed by the sizes.
+// With WT = 1 and no cluster a lane walks its channels alone and steps 1 and 2 fall away.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "layers.cuh"
+#include "math.cuh"
+
+namespace hmc {
+namespace recur {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256;
+constexpr int kWarps = 8;
+constexpr int kMaxCluster = 8;
+
+template <class C> struct alignas(2 * sizeof(C)) Step {
+    C a, b;
+};
+
+// A step applied to the value before it. From 0 it gives b whatever a is: a product of gates that has overflowed must
+// not turn a state of zero into NaN (a NaN or infinite gate shows in b already).
+template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return v == C(0) ? s.b : m_fma(s.a, v, s.b); }
+
+// Rows and channels of one operand, in elements; t may be negative.
+struct Walk {
+    int64_t b, t, c;
+};
+
+// The gate in one register: min(a, 1 - a) with the sign bit set where a is the larger part, so that both a and 1 - a
+// come out with full relative precision however close to 0 or 1 a is.
+template <class C, bool FAST> __device__ __forceinline__ C sigmoid_code(C g) {
+    C m;
+    if constexpr (FAST) {
+        // rounded to at most 11 bits later; e in (0, 1], so neither approximation leaves its range
+        float e, r;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.44269504088896341f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+        m = e * r;
+    } else {
+        const C e = exp(-m_abs(g));
+        m = e / (C(1) + e);
+    }
+    return g > C(0) ? -m : m;
+}
+__device__ __forceinline__ bool negative(float v) { return __float_as_int(v) < 0; }
+__device__ __forceinline__ bool negative(double v) { return __double2hiint(v) < 0; }
+// a and 1 - a of a gate: SIG: its code, otherwise its value.
+template <bool SIG, class C> __device__ __forceinline__ C kept(C m) {
+    if constexpr (SIG) return negative(m) ? C(1) + m : m;
+    else return m;
+}
+template <bool SIG, class C> __device__ __forceinline__ C left(C m) {
+    if constexpr (SIG) return negative(m) ? -m : C(1) - m;
+    else return C(1) - m;
+}
+template <bool SIG, class T> __device__ __forceinline__ typename Comp<T>::C gate_code(T g) {
+    using C = typename Comp<T>::C;
+    if constexpr (SIG) return sigmoid_code<C, sizeof(T) == 2>(up(g));
+    else return up(g);
+}
+
+// V elements at p, the channels `c` elements apart (V > 1 only where c is 1 and the access aligned).
+template <class T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
+    return *reinterpret_cast<const Pack<T, V> *>(p);
+}
+template <class T, int V> __device__ __forceinline__ void store_pack(T *p, const typename Comp<T>::C (&v)[V]) {
+    Pack<T, V> r;
+    if constexpr (V % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) down2(r.v[i], r.v[i + 1], v[i], v[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = down<T>(v[i]);
+    }
+    *reinterpret_cast<Pack<T, V> *>(p) = r;
+}
+
+// What a launch looks like; see plan_launch.
+struct Shape {
+    int32_t warps_time;  // WT
+    int32_t cluster;
+    int64_t tiles;       // channel tiles of 8 / WT * 32 * V channels
+    int64_t items;       // batch * tiles
+    unsigned grid;
+};
+
+// WT and the cluster grow until the launch has about sixteen warps an SM, but not beyond what the time axis can feed. The
+// constant is B200's SM count, not the device's, so that the order of folding is the same everywhere.
+inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, int v, int rows) {
+    constexpr int64_t kEnough = 148 * 16;
+    Shape s{1, 1, 0, 0, 0};
+    const int64_t warps = batch * ceil_div(channels, int64_t{32} * v);  // (both counts are below 2^62 / (32 v))
+    int64_t have = warps;
+    while (have < kEnough && s.warps_time < kWarps && static_cast<int64_t>(s.warps_time) * rows < time) {
+        s.warps_time *= 2;
+        have *= 2;
+    }
+    while (have < kEnough && s.warps_time == kWarps && s.cluster < kMaxCluster &&
+           static_cast<int64_t>(s.warps_time) * s.cluster * rows < time) {
+        s.cluster *= 2;
+        have *= 2;
+    }
+    s.tiles = ceil_div(channels, int64_t{32} * v * (kWarps / s.warps_time));
+    s.items = batch * s.tiles;
+    const int64_t most = (int64_t{1} << 30) / s.cluster;
+    s.grid = static_cast<unsigned>((s.items < most ? s.items : most) * s.cluster);
+    return s;
+}
+
+// ---- checks of the entry points ----
+inline hmc_status check_recurrence(const hmc_tensor_desc *gate, int32_t flags, int64_t *count) {
+    hmc_status s = check_desc(gate, "the gate");
+    if (s != HMC_OK) return s;
+    if (!dtype_is_float(gate->dtype)) return fail(HMC_INVALID, "a linear recurrence needs floating point tensors");
+    if (flags & ~(HMC_RECURRENCE_SIGMOID | HMC_RECURRENCE_COMPLEMENT | HMC_RECURRENCE_REVERSE)) {
+        return fail(HMC_INVALID, "unknown flags of a linear recurrence");
+    }
+    s = check_layer(gate, "the gate", gate->dtype, 3, gate->sizes, Use::kInput);
+    if (s != HMC_OK) return s;
+    s = count_layer(gate->sizes, 3, count);
+    if (s != HMC_OK) return s;
+    const int64_t states[2] = {gate->sizes[0], gate->sizes[2]};
+    int64_t ignored = 0;
+    return count_layer(states, 2, &ignored);
+}
+inline hmc_status check_state(const hmc_tensor_desc *d, const char *what, const hmc_tensor_desc *gate, Use use) {
+    if (d == nullptr) return HMC_OK;
+    const int64_t sizes[2] = {gate->sizes[0], gate->sizes[2]};
+    return check_layer(d, what, gate->dtype == HMC_F64 ? HMC_F64 : HMC_F32, 2, sizes, use);
+}
+
+// [batch, time, channels] in the order the rows are processed: from the last row on where that runs `backwards`.
+template <class P> inline Walk walk_rows(const hmc_tensor_desc *d, bool backwards, P *base) {
+    if (d == nullptr) return Walk{0, 0, 0};
+    Walk w{d->strides[0], d->strides[1], d->strides[2]};
+    if (backwards && d->sizes[1] > 0) {
+        *base += (d->sizes[1] - 1) * w.t * element_size(d->dtype);
+        w.t = -w.t;
+    }
+    return w;
+}
+inline Walk walk_state(const hmc_tensor_desc *d) { return d == nullptr ? Walk{0, 0, 0} : Walk{d->strides[0], 0, d->strides[1]}; }
+
+template <class Kernel, class Args>
+hmc_status launch(hmc_context_t ctx, Kernel kernel, const Shape &shape, const Args &args, const char *what) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(shape.grid);
+    config.blockDim = dim3(kThreads);
+    config.stream = ctx->stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = static_cast<unsigned>(shape.cluster);
+    attribute[0].val.clusterDim.y = 1;
+    attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = shape.cluster > 1 ? 1 : 0;
+    cudaError_t err = cudaLaunchKernelEx(&config, kernel, args);
+    if (err != cudaSuccess) return cuda_fail(err, what);
+    return HMC_OK;
+}
+
+// Where a warp stands: its item's batch and first channel, its place along the time axis.
+struct Place {
+    int lane, wt, wc;      // lane; the warp's place among the warps along time and along channels
+    int rank, cluster;     // the block's place in the cluster
+    int slot;              // lane's first column in the exchange arrays
+};
+template <int V> __device__ __forceinline__ Place place(int warps_time) {
+    Place p;
+    p.lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    p.wt = warp & (warps_time - 1);
+    p.wc = warp / warps_time;
+    cg::cluster_group cluster = cg::this_cluster();
+    p.rank = static_cast<int>(cluster.block_rank());
+    p.cluster = static_cast<int>(cluster.num_blocks());
+    p.slot = p.lane * V;
+    return p;
+}
+
+// Shared memory of the exchange, two generations so that one barrier a round is enough: a generation is written again
+// two rounds later, after the barrier of the round between, which every reader has reached by then.
+template <class C, int V> struct Exchange {
+    Step<C> warp[2][kWarps][32 * V];
+    Step<C> block[2][kMaxCluster][32 * V];
+};
+
+// Step 2 and the folds of step 3: `mine` is what this lane's rows do; v enters as the round's carry and leaves as the
+// value before this lane's rows; carry leaves as the value after the round.
+template <class C, int V>
+__device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, int generation, const Step<C> (&mine)[V],
+                                         C (&v)[V], C (&carry)[V]) {
+    Step<C>(&warps)[kWarps][32 * V] = x.warp[generation];
+    const int first = p.wc * warps_time;
+#pragma unroll
+    for (int i = 0; i < V; ++i) warps[first + p.wt][p.slot + i] = mine[i];
+    __syncthreads();
+    if (p.cluster > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        // (a cluster is used with all eight warps along time only, so a block has one tile of channels; warp w brings the
+        // block's fold to block w)
+        if (p.wt < p.cluster) {
+            Step<C>(*there)[32 * V] = cluster.map_shared_rank(x.block[generation], p.wt);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                Step<C> t = warps[0][p.slot + i];
+#pragma unroll 2
+                for (int w = 1; w < kWarps; ++w) {
+                    const Step<C> s = warps[w][p.slot + i];
+                    t.b = fold(s, t.b);
+                    t.a *= s.a;
+                }
+                there[p.rank][p.slot + i] = t;
+            }
+        }
+        cluster.sync();
+#pragma unroll 2
+        for (int k = 0; k < p.cluster; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                carry[i] = fold(x.block[generation][k][p.slot + i], carry[i]);
+                if (k < p.rank) v[i] = carry[i];
+            }
+        }
+#pragma unroll 2
+        for (int w = 0; w < p.wt; ++w) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = fold(warps[w][p.slot + i], v[i]);
+        }
+    } else {
+#pragma unroll 2
+        for (int w = 0; w < warps_time; ++w) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                carry[i] = fold(warps[first + w][p.slot + i], carry[i]);
+                if (w < p.wt) v[i] = carry[i];
+            }
+        }
+    }
+}
+
+}  // namespace recur
+}  // namespace hmc

@@ -76,6 +76,10 @@ HMC_MEM_OK = 0
 HMC_MEM_OUT_OF_MEMORY = 1
 HMC_MEM_FAILED = 2
 HMC_COMM_ID_BYTES = 128
+HMC_RECURRENCE_SIGMOID = 1
+HMC_RECURRENCE_COMPLEMENT = 2
+HMC_RECURRENCE_REVERSE = 4
+HMC_ACTIVATION_NONE = -1
 
 
 class hmc_device_properties(Structure):
@@ -259,6 +263,12 @@ FUNCTIONS = {
     "hmc_comm_allgather": (c_int32, [(c_void_p, "comm"), (c_void_p, "send"), (c_void_p, "recv"), (c_uint64, "bytes")]),
     "hmc_comm_wait": (c_int32, [(c_void_p, "comm")]),
     "hmc_comm_abort": (c_int32, [(c_void_p, "comm")]),
+    "hmc_linear_recurrence": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "out"), (POINTER(hmc_tensor_desc), "gate"), (POINTER(hmc_tensor_desc), "x"), (POINTER(hmc_tensor_desc), "initial"), (POINTER(hmc_tensor_desc), "last"), (c_int32, "flags")]),
+    "hmc_linear_recurrence_backward": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "dgate"), (POINTER(hmc_tensor_desc), "dx"), (POINTER(hmc_tensor_desc), "dinitial"), (POINTER(hmc_tensor_desc), "gate"), (POINTER(hmc_tensor_desc), "x"), (POINTER(hmc_tensor_desc), "out"), (POINTER(hmc_tensor_desc), "initial"), (POINTER(hmc_tensor_desc), "dout"), (POINTER(hmc_tensor_desc), "dlast"), (c_int32, "flags")]),
+    "hmc_group_norm_workspace": (c_int32, [(POINTER(hmc_tensor_desc), "src"), (c_int32, "groups"), (c_int32, "backward"), (POINTER(c_int64), "bytes")]),
+    "hmc_group_norm": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "out"), (POINTER(hmc_tensor_desc), "src"), (POINTER(hmc_tensor_desc), "weight"), (POINTER(hmc_tensor_desc), "bias"), (POINTER(hmc_tensor_desc), "mean"), (POINTER(hmc_tensor_desc), "rstd"), (c_int32, "groups"), (c_double, "eps"), (c_int32, "activation"), (c_void_p, "workspace"), (c_int64, "workspace_bytes")]),
+    "hmc_group_norm_backward": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "dsrc"), (POINTER(hmc_tensor_desc), "dweight"), (POINTER(hmc_tensor_desc), "dbias"), (POINTER(hmc_tensor_desc), "src"), (POINTER(hmc_tensor_desc), "dout"), (POINTER(hmc_tensor_desc), "mean"), (POINTER(hmc_tensor_desc), "rstd"), (POINTER(hmc_tensor_desc), "weight"), (POINTER(hmc_tensor_desc), "bias"), (c_int32, "groups"), (c_int32, "activation"), (c_void_p, "workspace"), (c_int64, "workspace_bytes")]),
+    "hmc_dropout": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "out"), (POINTER(hmc_tensor_desc), "src"), (POINTER(hmc_tensor_desc), "residual"), (c_double, "p"), (c_uint64, "seed"), (c_uint64, "offset")]),
 }
 
 

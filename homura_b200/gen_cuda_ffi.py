@@ -16,7 +16,7 @@ from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent.parent
 HEADERS = [ROOT / "include" / "homura_cuda.h", ROOT / "include" / "homura_cuda_alloc.h",
-           ROOT / "include" / "homura_cuda_shard.h"]
+           ROOT / "include" / "homura_cuda_shard.h", ROOT / "include" / "homura_cuda_layers.h"]
 OUT = Path(__file__).resolve().parent / "ffi.py"
 
 CTYPES = {

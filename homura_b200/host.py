@@ -820,6 +820,90 @@ class CudaBackend:
         (o, s), n, so, si = ln
         self._check(self.lib.hmc_exclusive_cumprod(self.ctx, o, s, n, so, si, int(bool(reverse))))
 
+    # ---- the operators of a recurrent sequence block (include/homura_cuda_layers.h) ----
+    def linear_recurrence(self, out: TensorData, gate: TensorData, x: TensorData, initial: Optional[TensorData] = None,
+                          last: Optional[TensorData] = None, *, sigmoid: bool = False, complement: bool = False,
+                          reverse: bool = False) -> None:
+        """h_t = a_t * h_{t-1} + u_t along dimension 1 of [batch, time, channels] into `out`, with a = gate or (sigmoid)
+        sigmoid(gate) and u = x or (complement) (1 - a) * x; from the state `initial` ([batch, channels], F32, or F64 for
+        F64 tensors; zeros when None), the state after the last step into `last`. `out` may be the view `x` or `gate`,
+        `last` the view `initial`. One step (time 1) is the form for generating a token."""
+        self._check(self.lib.hmc_linear_recurrence(
+            self.ctx, plain_desc("linear_recurrence", out), plain_desc("linear_recurrence", gate), plain_desc("linear_recurrence", x),
+            plain_desc("linear_recurrence", initial), plain_desc("linear_recurrence", last),
+            recurrence_flags(sigmoid, complement, reverse)))
+
+    def linear_recurrence_backward(self, dgate: TensorData, dx: TensorData, gate: TensorData, x: Optional[TensorData],
+                                   out: TensorData, dout: TensorData, initial: Optional[TensorData] = None,
+                                   dlast: Optional[TensorData] = None, dinitial: Optional[TensorData] = None, *,
+                                   sigmoid: bool = False, complement: bool = False, reverse: bool = False) -> None:
+        """The gradients of :meth:`linear_recurrence` into `dgate`, `dx` and (unless None) `dinitial`, from its operands,
+        its result `out`, and the gradients `dout` and `dlast` (zeros when None). `x` is read with `complement` only."""
+        k = "linear_recurrence_backward"
+        self._check(self.lib.hmc_linear_recurrence_backward(
+            self.ctx, plain_desc(k, dgate), plain_desc(k, dx), plain_desc(k, dinitial), plain_desc(k, gate), plain_desc(k, x),
+            plain_desc(k, out), plain_desc(k, initial), plain_desc(k, dout), plain_desc(k, dlast),
+            recurrence_flags(sigmoid, complement, reverse)))
+
+    def _group_norm_workspace(self, src, groups: int, backward: int) -> tuple:
+        """(storage to keep until the call is queued, its address or None, its bytes)."""
+        nbytes = ctypes.c_int64()
+        self._check(self.lib.hmc_group_norm_workspace(src, groups, backward, ctypes.byref(nbytes)))
+        ws = self.workspace(nbytes.value)
+        return ws, (ws.ptr if ws else None), nbytes.value
+
+    def group_norm(self, out: TensorData, src: TensorData, groups: int, weight: Optional[TensorData] = None,
+                   bias: Optional[TensorData] = None, mean: Optional[TensorData] = None, rstd: Optional[TensorData] = None, *,
+                   eps: float = 1e-5, activation: Optional[str] = None) -> None:
+        """act((src - mean) * rstd * weight + bias) over groups of neighbouring channels of a channels-last tensor
+        [samples, ..., channels], one mean and rstd per sample and group over all its positions, which `mean` and `rstd`
+        ([samples, groups], F32, or F64 for F64 tensors) receive for the backward pass. `activation`: None, "relu", "silu",
+        "gelu" or "gelu_tanh". `weight` and `bias` ([channels]) have src's dtype or F32. `out` may be the view `src`."""
+        k = "group_norm"
+        s = channels_last_desc(k, src)
+        ws, ptr, nbytes = self._group_norm_workspace(s, groups, 0)
+        self._check(self.lib.hmc_group_norm(self.ctx, channels_last_desc(k, out), s, plain_desc(k, weight), plain_desc(k, bias),
+                                            plain_desc(k, mean), plain_desc(k, rstd), groups, float(eps),
+                                            activation_code(activation), ptr, nbytes))
+
+    def group_norm_backward(self, dsrc: TensorData, src: TensorData, dout: TensorData, mean: TensorData, rstd: TensorData,
+                            groups: int, weight: Optional[TensorData] = None, bias: Optional[TensorData] = None,
+                            dweight: Optional[TensorData] = None, dbias: Optional[TensorData] = None, *,
+                            activation: Optional[str] = None) -> None:
+        """The gradients of :meth:`group_norm` into `dsrc` and (unless None) `dweight` and `dbias`, from its operands, the
+        moments it left and the gradient `dout`. `dsrc` may be the view `dout` or `src`."""
+        k = "group_norm_backward"
+        s = channels_last_desc(k, src)
+        ws, ptr, nbytes = self._group_norm_workspace(s, groups, 1)
+        self._check(self.lib.hmc_group_norm_backward(
+            self.ctx, channels_last_desc(k, dsrc), plain_desc(k, dweight), plain_desc(k, dbias), s, channels_last_desc(k, dout),
+            plain_desc(k, mean), plain_desc(k, rstd), plain_desc(k, weight), plain_desc(k, bias), groups,
+            activation_code(activation), ptr, nbytes))
+
+    def dropout(self, out: TensorData, src: TensorData, gen: "Generator", p: float,
+                residual: Optional[TensorData] = None) -> tuple:
+        """out = (residual +) src with every element dropped with probability p and the kept ones divided by 1 - p. The
+        mask is a function of the returned (seed, first block) and of the element's row-major position: hand the pair to
+        :meth:`dropout_backward`. `out` may be the view `src` or `residual`."""
+        state = gen.reserve(-(-src.numel // 4))
+        self._dropout("dropout", out, src, residual, p, state)
+        return state
+
+    def dropout_backward(self, dsrc: TensorData, dout: TensorData, p: float, state: tuple) -> None:
+        """The gradient of :meth:`dropout` with respect to its input, from the pair it returned (that with respect to the
+        residual is dout itself)."""
+        self._dropout("dropout_backward", dsrc, dout, None, p, state)
+
+    def _dropout(self, kernel: str, out: TensorData, src: TensorData, residual: Optional[TensorData], p: float, state: tuple) -> None:
+        operands = [out, src] if residual is None else [out, src, residual]
+        if out.numel == 0 or any(t.shape != out.shape for t in operands):
+            d = [plain_desc(kernel, t) for t in operands]  # nothing to write, or refused by the library
+        elif all(t.is_contiguous() for t in operands):
+            d = [_flat_desc(t) for t in operands]
+        else:
+            d = descs(kernel, operands)
+        self._check(self.lib.hmc_dropout(self.ctx, d[0], d[1], d[2] if len(d) > 2 else None, float(p), *state))
+
     def adamw_step(self, param: TensorData, grad: TensorData, exp_avg: TensorData, exp_avg_sq: TensorData, *,
                    lr: float, beta1: float, beta2: float, eps: float, weight_decay: float, step: float) -> None:
         """The fused AdamW update (hmc_adamw_step) with the scalars homura's optimizer derives
@@ -884,6 +968,56 @@ class AdamWGroup:
         if out.size:
             self.be._check(self.be.lib.hmc_copy_to_host(self.be.ctx, out.ctypes.data, self.grad_sq.ptr, out.nbytes))
         return out
+
+
+def plain_desc(kernel: str, t: Optional[TensorData]) -> Optional[hmc_tensor_desc]:
+    """The description of a tensor dimension by dimension, none merged or dropped; None stays None."""
+    if t is None:
+        return None
+    n = len(t.shape)
+    if n > MAX_DIMS:
+        raise BackendError(ffi.HMC_INVALID, f"{kernel} on CUDA supports at most {MAX_DIMS} dimensions, got {n}")
+    if CHECK_REACH:
+        check_reach(kernel, t, t.offset, [(size, [st]) for size, st in zip(t.shape, t.strides)], 0)
+    d = hmc_tensor_desc()
+    d.data, d.offset, d.dtype, d.ndim = t.storage.address, t.offset, t.dtype, n
+    d.sizes[:n] = t.shape
+    d.strides[:n] = t.strides
+    return d
+
+
+def channels_last_desc(kernel: str, t: TensorData) -> hmc_tensor_desc:
+    """[samples, ..., channels] as three dimensions, the ones between them merged into positions."""
+    n = len(t.shape)
+    if n == 3:
+        return plain_desc(kernel, t)
+    if n < 2:
+        raise BackendError(ffi.HMC_INVALID, f"{kernel} needs [samples, ..., channels], got {n} dimensions")
+    between = merge_dims(t.shape[1:-1], [t.strides[1:-1]])
+    if between is None:
+        between = [(0, [0])]
+    elif not between:
+        between = [(1, [0])]
+    if len(between) > 1:
+        raise BackendError(ffi.HMC_INVALID, f"{kernel}: the positions of a tensor of shape {tuple(t.shape)} and strides "
+                                            f"{tuple(t.strides)} are not evenly spaced")
+    size, (stride,) = between[0]
+    return plain_desc(kernel, TensorData(t.storage, t.dtype, (t.shape[0], size, t.shape[-1]), (t.strides[0], stride, t.strides[-1]), t.offset))
+
+
+def recurrence_flags(sigmoid: bool, complement: bool, reverse: bool) -> int:
+    return ((ffi.HMC_RECURRENCE_SIGMOID if sigmoid else 0) | (ffi.HMC_RECURRENCE_COMPLEMENT if complement else 0) |
+            (ffi.HMC_RECURRENCE_REVERSE if reverse else 0))
+
+
+ACTIVATIONS = {None: ffi.HMC_ACTIVATION_NONE, "relu": ffi.HMC_UNARY_RELU, "silu": ffi.HMC_UNARY_SILU,
+               "gelu": ffi.HMC_UNARY_GELU, "gelu_tanh": ffi.HMC_UNARY_GELU_TANH}
+
+
+def activation_code(activation: Optional[str]) -> int:
+    if activation not in ACTIVATIONS:
+        raise BackendError(ffi.HMC_INVALID, f"group norm's activation is one of {list(ACTIVATIONS)}, got {activation!r}")
+    return ACTIVATIONS[activation]
 
 
 def around(kernel: str, operands: Sequence[TensorData], shape: Sequence[int], dim: int):
