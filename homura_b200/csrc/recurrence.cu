@@ -15,12 +15,16 @@ struct ForwardArgs {
     int32_t warps_time;
 };
 
-template <class T, int V> constexpr int kResident = sizeof(T) == 8 ? 2 : (V == 2 ? 3 : 4);
+constexpr int kStages = 3;
 
-template <class T, int V, int R, bool SIG, bool COMP>
-__global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(const __grid_constant__ ForwardArgs a) {
+template <class T, int V, int R, int COPY, bool SIG, bool COMP>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kernel(const __grid_constant__ ForwardArgs a) {
     using C = typename Comp<T>::C;
+    using G = Ring<T, V, COPY>;
     __shared__ Exchange<C, V> shared;
+    extern __shared__ __align__(16) unsigned char memory[];
+    constexpr int kStage = 2 * R * G::kRow;  // a warp's gates, then its x
+    unsigned char *ring = memory + (threadIdx.x >> 5) * (kStages * kStage);
     const Place p = place<V>(a.warps_time);
     const bool alone = a.warps_time == 1 && p.cluster == 1;
     const int64_t round = static_cast<int64_t>(R) * a.warps_time * p.cluster;
@@ -29,11 +33,14 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(cons
     int generation = 0;
     for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
         const int64_t batch = item / a.tiles;
-        const int64_t channel = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V) + p.slot;
+        const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
+        const int64_t channel = tile + p.slot;
         const bool live = channel < a.channels;
-        const int64_t rows = live ? a.time : 0;
-        const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + channel * a.wgate.c;
-        const T *x = reinterpret_cast<const T *>(a.x) + batch * a.wx.b + channel * a.wx.c;
+        // what this lane loads or copies: its own channels, or its part of a row
+        const int64_t column = COPY > 0 ? tile + G::channel() : channel;
+        const bool loads = column < a.channels;
+        const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + column * a.wgate.c;
+        const T *x = reinterpret_cast<const T *>(a.x) + batch * a.wx.b + column * a.wx.c;
         T *out = reinterpret_cast<T *>(a.out) + batch * a.wout.b + channel * a.wout.c;
         C carry[V];
 #pragma unroll
@@ -42,13 +49,16 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(cons
             if (a.initial != nullptr && live)
                 carry[i] = reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
         }
-        // rows of this lane from t0 on that exist, R at most
-        auto count = [&](int64_t t0) { return static_cast<int>(rows - t0 < R ? (rows - t0 > 0 ? rows - t0 : 0) : R); };
-        for (int64_t base = 0; base < a.time; base += round) {
-            const int64_t t0 = base + mine;
-            const int n = count(t0);
-            Pack<T, V> rg[R], rx[R];
-            {
+        // rows of this warp from t0 on that exist, R at most
+        const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
+        Pack<T, V> rg[R], rx[R];
+        const auto fetch = [&](int64_t t0, int stage) {
+            const int n = loads ? count(t0) : 0;
+            if constexpr (COPY > 0) {
+                copy_rows<T, V, COPY, R>(ring + stage * kStage, 0, gate + (t0 + G::row()) * a.wgate.t, a.wgate.t, n);
+                copy_rows<T, V, COPY, R>(ring + stage * kStage, R, x + (t0 + G::row()) * a.wx.t, a.wx.t, n);
+                async_copy_commit();
+            } else {
                 const T *pg = gate + t0 * a.wgate.t, *px = x + t0 * a.wx.t;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -60,29 +70,58 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(cons
                     px += a.wx.t;
                 }
             }
+        };
+        int stage = 0;
+        if constexpr (COPY > 0) {
+#pragma unroll
+            for (int k = 0; k + 1 < kStages; ++k) fetch(mine + k * round, k);
+        }
+        for (int64_t base = 0; base < a.time; base += round) {
+            const int64_t t0 = base + mine;
+            const int n = count(t0);
+            if constexpr (COPY > 0) {
+                // the stage of the round before is free: the copies of kStages - 1 rounds are on their way
+                __syncwarp();
+                fetch(t0 + (kStages - 1) * round, stage == 0 ? kStages - 1 : stage - 1);
+                wait_for_all_but<kStages - 1>();
+                __syncwarp();
+                const unsigned char *from = ring + stage * kStage + p.lane * static_cast<int>(sizeof(T) * V);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    rg[r] = load_pack<T, V>(reinterpret_cast<const T *>(from + r * G::kRow));
+                    rx[r] = load_pack<T, V>(reinterpret_cast<const T *>(from + (R + r) * G::kRow));
+                }
+                stage = stage + 1 == kStages ? 0 : stage + 1;
+            } else {
+                fetch(t0, 0);
+            }
+            // All R rows exist for most warps (`whole`, the same for a warp's lanes): that form has no conditions in it. The
+            // barriers of the exchange stand outside. Lanes beyond the last channel compute on whatever their registers
+            // hold and write nothing.
             C ca[R][V], cu[R][V];
+            Step<C> s[V];
+            const auto read = [&](auto whole) {
+                constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+                for (int r = 0; r < R; ++r) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    ca[r][i] = C(1);
-                    cu[r][i] = C(0);
-                    if (r < n) {
-                        const C m = gate_code<SIG>(rg[r].v[i]);
-                        ca[r][i] = kept<SIG>(m);
-                        cu[r][i] = COMP ? left<SIG>(m) * up(rx[r].v[i]) : up(rx[r].v[i]);
+                    for (int i = 0; i < V; ++i) {
+                        const Gate<C> g = gate_of<SIG>(rg[r].v[i]);
+                        ca[r][i] = kWhole || r < n ? g.a : C(1);
+                        cu[r][i] = kWhole || r < n ? (COMP ? g.rest * up(rx[r].v[i]) : up(rx[r].v[i])) : C(0);
                     }
                 }
-            }
+            };
+            if (n == R) read(std::true_type{});
+            else read(std::false_type{});
             C h[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = carry[i];
             if (!alone) {
-                Step<C> s[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     s[i].a = ca[0][i];
-                    s[i].b = cu[0][i];
+                    s[i].b = m_fma(ca[0][i], C(0), cu[0][i]);
 #pragma unroll
                     for (int r = 1; r < R; ++r) {
                         s[i].b = m_fma(ca[r][i], s[i].b, cu[r][i]);
@@ -92,23 +131,28 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(cons
                 exchange(shared, p, a.warps_time, generation, s, h, carry);
                 generation ^= 1;
             }
-            T *po = out + t0 * a.wout.t;
+            const auto write = [&](auto whole) {
+                constexpr bool kWhole = decltype(whole)::value;
+                T *po = out + t0 * a.wout.t;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (r < n) {
+                for (int r = 0; r < R; ++r) {
+                    if (kWhole || r < n) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) h[i] = m_fma(ca[r][i], h[i], cu[r][i]);
-                    store_pack<T, V>(po, h);
+                        for (int i = 0; i < V; ++i) h[i] = m_fma(ca[r][i], h[i], cu[r][i]);
+                        if (live) store_pack<T, V>(po, h);
+                    }
+                    po += a.wout.t;
                 }
-                po += a.wout.t;
-            }
-            if (n > 0 && t0 + n == a.time && a.last != nullptr) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = h[i];
-            }
+            };
+            if (n == R) write(std::true_type{});
+            else write(std::false_type{});
             if (alone) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) carry[i] = h[i];
+            }
+            if (a.last != nullptr && live && n > 0 && t0 + n == a.time) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = h[i];
             }
         }
         if (a.time == 0 && live && p.rank == 0 && p.wt == 0 && a.last != nullptr) {
@@ -118,19 +162,19 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) forward_kernel(cons
     }
 }
 
-template <class T, int V, int R>
+template <class T, int V, int R, int COPY>
 hmc_status launch_forward(hmc_context_t ctx, ForwardArgs &a, int64_t batch, int32_t flags) {
     const Shape shape = plan_launch(batch, a.time, a.channels, V, R);
     a.tiles = shape.tiles;
     a.items = shape.items;
     a.warps_time = shape.warps_time;
-    const char *what = "linear recurrence kernel launch";
-    switch (flags & (HMC_RECURRENCE_SIGMOID | HMC_RECURRENCE_COMPLEMENT)) {
-        case 0: return launch(ctx, forward_kernel<T, V, R, false, false>, shape, a, what);
-        case HMC_RECURRENCE_SIGMOID: return launch(ctx, forward_kernel<T, V, R, true, false>, shape, a, what);
-        case HMC_RECURRENCE_COMPLEMENT: return launch(ctx, forward_kernel<T, V, R, false, true>, shape, a, what);
-        default: return launch(ctx, forward_kernel<T, V, R, true, true>, shape, a, what);
-    }
+    constexpr int kShared = COPY > 0 ? kWarps * kStages * 2 * R * Ring<T, V, COPY>::kRow : 0;
+    const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
+        static bool raised[kKnownDevices] = {};
+        return launch(ctx, forward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, raised, kShared, shape, a,
+                      "linear recurrence kernel launch");
+    };
+    return dispatch_flags(flags, go);
 }
 
 }  // namespace
@@ -171,12 +215,15 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
         a.time = time;
         a.channels = channels;
         const bool pairs = layer_vectors(out, 4) && layer_vectors(gate, 4) && layer_vectors(x, 4);
+        const bool wide = layer_vectors(gate, 16) && layer_vectors(x, 16) && layer_vectors(out, 4);
         return dispatch_float(dt, [&](auto tag) -> hmc_status {
             using T = decltype(tag);
+            constexpr int kWord = sizeof(T) == 8 ? 8 : 4, V = sizeof(T) == 2 ? 2 : 1;
             if constexpr (sizeof(T) == 2) {
-                if (pairs) return time == 1 ? launch_forward<T, 2, 1>(ctx, a, batch, flags) : launch_forward<T, 2, 8>(ctx, a, batch, flags);
+                if (!pairs) return time == 1 ? launch_forward<T, 1, 1, 0>(ctx, a, batch, flags) : launch_forward<T, 1, 8, 0>(ctx, a, batch, flags);
             }
-            return time == 1 ? launch_forward<T, 1, 1>(ctx, a, batch, flags) : launch_forward<T, 1, 8>(ctx, a, batch, flags);
+            if (time == 1) return launch_forward<T, V, 1, 0>(ctx, a, batch, flags);
+            return wide ? launch_forward<T, V, 8, 16>(ctx, a, batch, flags) : launch_forward<T, V, 8, kWord>(ctx, a, batch, flags);
         });
     });
 }

@@ -36,46 +36,39 @@ template <class C> struct alignas(2 * sizeof(C)) Step {
     C a, b;
 };
 
-// A step applied to the value before it. From 0 it gives b whatever a is: a product of gates that has overflowed must
-// not turn a state of zero into NaN (a NaN or infinite gate shows in b already).
-template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return v == C(0) ? s.b : m_fma(s.a, v, s.b); }
+// A step applied to the value before it.
+template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return m_fma(s.a, v, s.b); }
+// A product of gates that has overflowed is held at the largest finite number, so that a state of zero before it stays
+// zero instead of becoming NaN. (A NaN or infinite gate shows in b already, which is folded from zero.)
+__device__ __forceinline__ float finite(float a) { return fminf(fmaxf(a, -3.4028234663852886e38f), 3.4028234663852886e38f); }
+__device__ __forceinline__ double finite(double a) { return fmin(fmax(a, -1.7976931348623157e308), 1.7976931348623157e308); }
 
 // Rows and channels of one operand, in elements; t may be negative.
 struct Walk {
     int64_t b, t, c;
 };
 
-// The gate in one register: min(a, 1 - a) with the sign bit set where a is the larger part, so that both a and 1 - a
-// come out with full relative precision however close to 0 or 1 a is.
-template <class C, bool FAST> __device__ __forceinline__ C sigmoid_code(C g) {
-    C m;
-    if constexpr (FAST) {
-        // rounded to at most 11 bits later; e in (0, 1], so neither approximation leaves its range
-        float e, r;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.44269504088896341f));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-        m = e * r;
-    } else {
-        const C e = exp(-m_abs(g));
-        m = e / (C(1) + e);
-    }
-    return g > C(0) ? -m : m;
-}
-__device__ __forceinline__ bool negative(float v) { return __float_as_int(v) < 0; }
-__device__ __forceinline__ bool negative(double v) { return __double2hiint(v) < 0; }
-// a and 1 - a of a gate: SIG: its code, otherwise its value.
-template <bool SIG, class C> __device__ __forceinline__ C kept(C m) {
-    if constexpr (SIG) return negative(m) ? C(1) + m : m;
-    else return m;
-}
-template <bool SIG, class C> __device__ __forceinline__ C left(C m) {
-    if constexpr (SIG) return negative(m) ? -m : C(1) - m;
-    else return C(1) - m;
-}
-template <bool SIG, class T> __device__ __forceinline__ typename Comp<T>::C gate_code(T g) {
+// a and 1 - a of a gate, each with full relative precision however close to 0 or 1 a is.
+template <class C> struct Gate {
+    C a, rest;
+};
+template <bool SIG, class T> __device__ __forceinline__ Gate<typename Comp<T>::C> gate_of(T stored) {
     using C = typename Comp<T>::C;
-    if constexpr (SIG) return sigmoid_code<C, sizeof(T) == 2>(up(g));
-    else return up(g);
+    const C g = up(stored);
+    if constexpr (!SIG) {
+        return Gate<C>{g, C(1) - g};
+    } else if constexpr (sizeof(T) == 2) {
+        // rounded to at most 11 bits later. e = exp(-g), held below 2^126 so that both approximations stay in range (a is
+        // 2^-126 then, where it should be less); the minimum passes a NaN on
+        float t = g * -1.44269504088896341f, e, a;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(t), "f"(126.0f));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
+        return Gate<C>{a, e * a};
+    } else {
+        const C e = exp(-m_abs(g)), large = C(1) / (C(1) + e), small = e * large;
+        return g > C(0) ? Gate<C>{large, small} : Gate<C>{small, large};
+    }
 }
 
 // V elements at p, the channels `c` elements apart (V > 1 only where c is 1 and the access aligned).
@@ -92,6 +85,41 @@ template <class T, int V> __device__ __forceinline__ void store_pack(T *p, const
         for (int i = 0; i < V; ++i) r.v[i] = down<T>(v[i]);
     }
     *reinterpret_cast<Pack<T, V> *>(p) = r;
+}
+
+// A warp's rows come through a ring in shared memory that its own asynchronous copies fill rounds ahead: no register
+// holds data in flight. A copy moves COPY bytes: 16 where every row begins on such a boundary, a quarter of the
+// instructions of the copies of one lane's word (4 or 8 bytes) that any layout allows. A warp waits for its own copies
+// only. Elements of 2 bytes that do not pair up (odd offsets or strides) are too small for an asynchronous copy and are
+// loaded to registers instead (COPY = 0), as is a single step.
+template <int BYTES> __device__ __forceinline__ void copy_async(void *shared_dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared_dst))), "l"(src), "n"(BYTES)
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_for_all_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <class T, int V, int COPY> struct Ring {
+    static constexpr int kRow = 32 * V * static_cast<int>(sizeof(T));  // bytes of a warp's row
+    static constexpr int kCopies = COPY > 0 ? kRow / COPY : 32;        // copies a row
+    static constexpr int kAtOnce = 32 / kCopies;                       // rows the warp copies with one instruction
+    static constexpr int kStep = COPY > 0 ? COPY / static_cast<int>(sizeof(T)) : V;  // elements a copy
+    // The row and the channel of the warp's rows that this lane copies.
+    __device__ __forceinline__ static int row() { return (threadIdx.x & 31) / kCopies; }
+    __device__ __forceinline__ static int channel() { return (threadIdx.x & 31) % kCopies * kStep; }
+};
+
+// `rows` rows into the ring from row `to` on, of which `there` exist; p: this lane's part of the first.
+template <class T, int V, int COPY, int ROWS>
+__device__ __forceinline__ void copy_rows(unsigned char *ring, int to, const T *p, int64_t stride, int there) {
+    using G = Ring<T, V, COPY>;
+    unsigned char *dst = ring + (to + G::row()) * G::kRow + G::channel() * static_cast<int>(sizeof(T));
+    const int64_t next = stride * G::kAtOnce;
+    static_assert(ROWS % G::kAtOnce == 0 || ROWS == 1, "whole instructions");
+#pragma unroll
+    for (int r = 0; r < ROWS; r += G::kAtOnce) {
+        if (r + G::row() < there) copy_async<COPY>(dst + r * G::kRow, p);
+        p += next;
+    }
 }
 
 // What a launch looks like; see plan_launch.
@@ -160,9 +188,30 @@ template <class P> inline Walk walk_rows(const hmc_tensor_desc *d, bool backward
 }
 inline Walk walk_state(const hmc_tensor_desc *d) { return d == nullptr ? Walk{0, 0, 0} : Walk{d->strides[0], 0, d->strides[1]}; }
 
+template <class F> hmc_status dispatch_flags(int32_t flags, F &&f) {
+    using Yes = std::true_type;
+    using No = std::false_type;
+    switch (flags & (HMC_RECURRENCE_SIGMOID | HMC_RECURRENCE_COMPLEMENT)) {
+        case 0: return f(No{}, No{});
+        case HMC_RECURRENCE_SIGMOID: return f(Yes{}, No{});
+        case HMC_RECURRENCE_COMPLEMENT: return f(No{}, Yes{});
+        default: return f(Yes{}, Yes{});
+    }
+}
+
+constexpr int kKnownDevices = 64;
+
+// `raised` remembers, per kernel and device, that the kernel may use its dynamic shared memory (a race between threads
+// only repeats the call).
 template <class Kernel, class Args>
-hmc_status launch(hmc_context_t ctx, Kernel kernel, const Shape &shape, const Args &args, const char *what) {
+hmc_status launch(hmc_context_t ctx, Kernel kernel, bool (&raised)[kKnownDevices], int shared, const Shape &shape, const Args &args,
+                  const char *what) {
+    if (shared > 0 && (ctx->device >= kKnownDevices || !raised[ctx->device])) {
+        HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared), what);
+        if (ctx->device < kKnownDevices) raised[ctx->device] = true;
+    }
     cudaLaunchConfig_t config{};
+    config.dynamicSmemBytes = static_cast<size_t>(shared);
     config.gridDim = dim3(shape.grid);
     config.blockDim = dim3(kThreads);
     config.stream = ctx->stream;
@@ -200,8 +249,8 @@ template <int V> __device__ __forceinline__ Place place(int warps_time) {
 // Shared memory of the exchange, two generations so that one barrier a round is enough: a generation is written again
 // two rounds later, after the barrier of the round between, which every reader has reached by then.
 template <class C, int V> struct Exchange {
-    Step<C> warp[2][kWarps][32 * V];
-    Step<C> block[2][kMaxCluster][32 * V];
+    alignas(16) Step<C> warp[2][kWarps][32 * V];
+    alignas(16) Step<C> block[2][kMaxCluster][32 * V];
 };
 
 // Step 2 and the folds of step 3: `mine` is what this lane's rows do; v enters as the round's carry and leaves as the
@@ -209,10 +258,16 @@ template <class C, int V> struct Exchange {
 template <class C, int V>
 __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, int generation, const Step<C> (&mine)[V],
                                          C (&v)[V], C (&carry)[V]) {
+    using Pair = Pack<Step<C>, V>;
     Step<C>(&warps)[kWarps][32 * V] = x.warp[generation];
+    const auto at = [&](const Step<C> (&row)[32 * V]) { return *reinterpret_cast<const Pair *>(&row[p.slot]); };
     const int first = p.wc * warps_time;
+    {
+        Pair mine_packed;
 #pragma unroll
-    for (int i = 0; i < V; ++i) warps[first + p.wt][p.slot + i] = mine[i];
+        for (int i = 0; i < V; ++i) mine_packed.v[i] = Step<C>{finite(mine[i].a), mine[i].b};
+        *reinterpret_cast<Pair *>(&warps[first + p.wt][p.slot]) = mine_packed;
+    }
     __syncthreads();
     if (p.cluster > 1) {
         cg::cluster_group cluster = cg::this_cluster();
@@ -220,38 +275,43 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
         // block's fold to block w)
         if (p.wt < p.cluster) {
             Step<C>(*there)[32 * V] = cluster.map_shared_rank(x.block[generation], p.wt);
+            Pair t = at(warps[0]);
+#pragma unroll 4
+            for (int w = 1; w < kWarps; ++w) {
+                const Pair s = at(warps[w]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                Step<C> t = warps[0][p.slot + i];
-#pragma unroll 2
-                for (int w = 1; w < kWarps; ++w) {
-                    const Step<C> s = warps[w][p.slot + i];
-                    t.b = fold(s, t.b);
-                    t.a *= s.a;
+                for (int i = 0; i < V; ++i) {
+                    t.v[i].b = fold(s.v[i], t.v[i].b);
+                    t.v[i].a *= s.v[i].a;
                 }
-                there[p.rank][p.slot + i] = t;
             }
+#pragma unroll
+            for (int i = 0; i < V; ++i) t.v[i].a = finite(t.v[i].a);
+            *reinterpret_cast<Pair *>(&there[p.rank][p.slot]) = t;
         }
         cluster.sync();
-#pragma unroll 2
+#pragma unroll 4
         for (int k = 0; k < p.cluster; ++k) {
+            const Pair s = at(x.block[generation][k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                carry[i] = fold(x.block[generation][k][p.slot + i], carry[i]);
+                carry[i] = fold(s.v[i], carry[i]);
                 if (k < p.rank) v[i] = carry[i];
             }
         }
-#pragma unroll 2
+#pragma unroll 4
         for (int w = 0; w < p.wt; ++w) {
+            const Pair s = at(warps[w]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = fold(warps[w][p.slot + i], v[i]);
+            for (int i = 0; i < V; ++i) v[i] = fold(s.v[i], v[i]);
         }
     } else {
-#pragma unroll 2
+#pragma unroll 4
         for (int w = 0; w < warps_time; ++w) {
+            const Pair s = at(warps[first + w]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                carry[i] = fold(warps[first + w][p.slot + i], carry[i]);
+                carry[i] = fold(s.v[i], carry[i]);
                 if (w < p.wt) v[i] = carry[i];
             }
         }

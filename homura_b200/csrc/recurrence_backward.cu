@@ -18,12 +18,18 @@ struct BackwardArgs {
     int32_t warps_time;
 };
 
-template <class T, int V> constexpr int kResident = sizeof(T) == 8 ? 1 : (V == 2 ? 2 : 3);
+constexpr int kStages = 2;
+template <int R, bool COMP> constexpr int kStageRows = (COMP ? 4 : 3) * R + 1;
 
-template <class T, int V, int R, bool SIG, bool COMP>
-__global__ void __launch_bounds__(kThreads, kResident<T, V>) backward_kernel(const __grid_constant__ BackwardArgs a) {
+template <class T, int V, int R, int COPY, bool SIG, bool COMP>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_kernel(const __grid_constant__ BackwardArgs a) {
     using C = typename Comp<T>::C;
+    using G = Ring<T, V, COPY>;
     __shared__ Exchange<C, V> shared;
+    extern __shared__ __align__(16) unsigned char memory[];
+    // a warp's rows of a stage: the gates (that of the row before first), dout, the states, x
+    constexpr int kGate = 0, kDout = R + 1, kState = 2 * R + 1, kX = 3 * R + 1, kStage = kStageRows<R, COMP> * G::kRow;
+    unsigned char *ring = memory + (threadIdx.x >> 5) * (kStages * kStage);
     const Place p = place<V>(a.warps_time);
     const bool alone = a.warps_time == 1 && p.cluster == 1;
     const int64_t round = static_cast<int64_t>(R) * a.warps_time * p.cluster;
@@ -32,13 +38,16 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) backward_kernel(con
     int generation = 0;
     for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
         const int64_t batch = item / a.tiles;
-        const int64_t channel = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V) + p.slot;
+        const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
+        const int64_t channel = tile + p.slot;
         const bool live = channel < a.channels;
-        const int64_t rows = live ? a.time : 0;
-        const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + channel * a.wgate.c;
-        const T *x = COMP ? reinterpret_cast<const T *>(a.x) + batch * a.wx.b + channel * a.wx.c : nullptr;
-        const T *out = reinterpret_cast<const T *>(a.out) + batch * a.wout.b + channel * a.wout.c;
-        const T *dout = reinterpret_cast<const T *>(a.dout) + batch * a.wdout.b + channel * a.wdout.c;
+        // what this lane loads or copies: its own channels, or its part of a row
+        const int64_t column = COPY > 0 ? tile + G::channel() : channel;
+        const bool loads = column < a.channels;
+        const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + column * a.wgate.c;
+        const T *x = COMP ? reinterpret_cast<const T *>(a.x) + batch * a.wx.b + column * a.wx.c : nullptr;
+        const T *out = reinterpret_cast<const T *>(a.out) + batch * a.wout.b + column * a.wout.c;
+        const T *dout = reinterpret_cast<const T *>(a.dout) + batch * a.wdout.b + column * a.wdout.c;
         T *dgate = reinterpret_cast<T *>(a.dgate) + batch * a.wdgate.b + channel * a.wdgate.c;
         T *dx = reinterpret_cast<T *>(a.dx) + batch * a.wdx.b + channel * a.wdx.c;
         C carry[V];
@@ -47,88 +56,132 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) backward_kernel(con
             carry[i] = C(0);
             if (a.dlast != nullptr && live) carry[i] = reinterpret_cast<const C *>(a.dlast)[batch * a.wdlast.b + (channel + i) * a.wdlast.c];
         }
-        for (int64_t base = 0; base < a.time; base += round) {
-            const int64_t t0 = base + mine;
-            // rows of this lane that exist; `last`: the last row in processing order is among them
-            const int n = static_cast<int>(rows - t0 < R ? (rows - t0 > 0 ? rows - t0 : 0) : R);
-            const bool last = n > 0 && t0 + n == a.time;
-            Pack<T, V> rg[R], rd[R], rh[R], rx[COMP ? R : 1], before;
-            {
-                const T *pg = gate + t0 * a.wgate.t, *pd = dout + t0 * a.wdout.t, *ph = out + (t0 + 1) * a.wout.t;
-                const T *px = COMP ? x + t0 * a.wx.t : nullptr;
-                if (n > 0 && t0 > 0) before = load_pack<T, V>(pg - a.wgate.t);
+        // rows of this warp from t0 on that exist, R at most
+        const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
+        Pack<T, V> direct[COPY > 0 ? 1 : kStageRows<R, COMP>];
+        const auto fetch = [&](int64_t t0, int stage) {
+            const int n = loads ? count(t0) : 0, states = loads ? count(t0 + 1) : 0, before = n > 0 && t0 > 0 ? 1 : 0;
+            if constexpr (COPY > 0) {
+                unsigned char *to = ring + stage * kStage;
+                const int64_t row = t0 + G::row();
+                copy_rows<T, V, COPY, 1>(to, kGate, gate + (row - 1) * a.wgate.t, a.wgate.t, before);
+                copy_rows<T, V, COPY, R>(to, kGate + 1, gate + row * a.wgate.t, a.wgate.t, n);
+                copy_rows<T, V, COPY, R>(to, kDout, dout + row * a.wdout.t, a.wdout.t, n);
+                copy_rows<T, V, COPY, R>(to, kState, out + (row + 1) * a.wout.t, a.wout.t, states);
+                if constexpr (COMP) copy_rows<T, V, COPY, R>(to, kX, x + row * a.wx.t, a.wx.t, n);
+                async_copy_commit();
+            } else {
+                if (before) direct[kGate] = load_pack<T, V>(gate + (t0 - 1) * a.wgate.t);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (r < n) {
-                        rg[r] = load_pack<T, V>(pg);
-                        rd[r] = load_pack<T, V>(pd);
-                        if constexpr (COMP) rx[r] = load_pack<T, V>(px);
-                        if (r + 1 < n || !last) rh[r] = load_pack<T, V>(ph);
+                        direct[kGate + 1 + r] = load_pack<T, V>(gate + (t0 + r) * a.wgate.t);
+                        direct[kDout + r] = load_pack<T, V>(dout + (t0 + r) * a.wdout.t);
+                        if (r < states) direct[kState + r] = load_pack<T, V>(out + (t0 + r + 1) * a.wout.t);
+                        if constexpr (COMP) direct[kX + r] = load_pack<T, V>(x + (t0 + r) * a.wx.t);
                     }
-                    pg += a.wgate.t;
-                    pd += a.wdout.t;
-                    ph += a.wout.t;
-                    if constexpr (COMP) px += a.wx.t;
                 }
             }
-            // the gates, in the code that gives both a and 1 - a; first: that of the row before this lane's
-            C first[V], m[R][V];
+        };
+        int filled = 0;
+        if constexpr (COPY > 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                first[i] = n > 0 && t0 > 0 ? kept<SIG>(gate_code<SIG>(before.v[i])) : C(1);
-#pragma unroll
-                for (int r = 0; r < R; ++r) m[r][i] = r < n ? gate_code<SIG>(rg[r].v[i]) : C(1);
+            for (int k = 0; k + 1 < kStages; ++k) fetch(mine + k * round, k);
+        }
+        for (int64_t base = 0; base < a.time; base += round) {
+            const int64_t t0 = base + mine;
+            const int n = count(t0);
+            const bool last = n > 0 && t0 + n == a.time;  // the last row in processing order is among this warp's
+            const int stage = filled;
+            if constexpr (COPY > 0) {
+                // the stage of the round before is free: the copies of kStages - 1 rounds are on their way
+                __syncwarp();
+                fetch(t0 + (kStages - 1) * round, stage == 0 ? kStages - 1 : stage - 1);
+                wait_for_all_but<kStages - 1>();
+                __syncwarp();
+                filled = stage + 1 == kStages ? 0 : stage + 1;
+            } else {
+                fetch(t0, 0);
             }
+            const unsigned char *from = ring + stage * kStage + p.lane * static_cast<int>(sizeof(T) * V);
+            const auto at = [&](int row) -> Pack<T, V> {
+                if constexpr (COPY > 0) return load_pack<T, V>(reinterpret_cast<const T *>(from + row * G::kRow));
+                else return direct[row];
+            };
+            // All R rows exist for most warps (`whole`, the same for a warp's lanes): that form has no conditions in it. The
+            // barriers of the exchange stand outside. Lanes beyond the last channel compute on whatever there is and write
+            // nothing.
+            C first[V];  // the gate of the row before this warp's
+            Gate<C> m[R][V];
+            Step<C> s[V];
+            const auto read = [&](auto whole) {
+                constexpr bool kWhole = decltype(whole)::value;
+                const Pack<T, V> before = at(kGate);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    first[i] = n > 0 && t0 > 0 ? gate_of<SIG>(before.v[i]).a : C(1);
+                    s[i] = Step<C>{first[i], C(0)};
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const Pack<T, V> g = at(kGate + 1 + r), d = at(kDout + r);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        if (kWhole || r < n) {
+                            m[r][i] = gate_of<SIG>(g.v[i]);
+                            const C c = r == 0 ? first[i] : m[r == 0 ? 0 : r - 1][i].a;
+                            s[i].b = m_fma(c, s[i].b, up(d.v[i]));
+                            if (r > 0) s[i].a *= c;
+                        }
+                    }
+                }
+            };
+            if (n == R) read(std::true_type{});
+            else read(std::false_type{});
             C g[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) g[i] = carry[i];
             if (!alone) {
-                Step<C> s[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s[i].a = first[i];
-                    s[i].b = n > 0 ? up(rd[0].v[i]) : C(0);
-#pragma unroll
-                    for (int r = 1; r < R; ++r) {
-                        if (r < n) {
-                            const C c = kept<SIG>(m[r - 1][i]);
-                            s[i].b = m_fma(c, s[i].b, up(rd[r].v[i]));
-                            s[i].a *= c;
-                        }
-                    }
-                }
                 exchange(shared, p, a.warps_time, generation, s, g, carry);
                 generation ^= 1;
             }
-            T *pg = dgate + t0 * a.wdgate.t, *px = dx + t0 * a.wdx.t;
+            const auto write = [&](auto whole) {
+                constexpr bool kWhole = decltype(whole)::value;  // (and the last row in processing order is not among them)
+                T *pg = dgate + t0 * a.wdgate.t, *px = dx + t0 * a.wdx.t;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (r < n) {
-                    C da[V], du[V];
+                for (int r = 0; r < R; ++r) {
+                    if (kWhole || r < n) {
+                        const Pack<T, V> d = at(kDout + r), state = at(kState + r), xr = at(COMP ? kX + r : kGate);
+                        C da[V], du[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        g[i] = m_fma(r == 0 ? first[i] : kept<SIG>(m[r - 1 < 0 ? 0 : r - 1][i]), g[i], up(rd[r].v[i]));
-                        C h;
-                        if (r + 1 == n && last) {
-                            h = a.initial == nullptr ? C(0)
-                                                     : reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
-                        } else {
-                            h = up(rh[r].v[i]);
+                        for (int i = 0; i < V; ++i) {
+                            g[i] = m_fma(r == 0 ? first[i] : m[r == 0 ? 0 : r - 1][i].a, g[i], up(d.v[i]));
+                            C h = up(state.v[i]);
+                            if constexpr (!kWhole) {
+                                if (r + 1 == n && last) {
+                                    h = a.initial == nullptr || !live ? C(0)
+                                                                      : reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
+                                    if (a.dinitial != nullptr && live) {
+                                        reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = m[r][i].a * g[i];
+                                    }
+                                }
+                            }
+                            if constexpr (COMP) h = h - up(xr.v[i]);
+                            du[i] = COMP ? g[i] * m[r][i].rest : g[i];
+                            da[i] = g[i] * h;
+                            if constexpr (SIG) da[i] = da[i] * (m[r][i].a * m[r][i].rest);
                         }
-                        if constexpr (COMP) h = h - up(rx[r].v[i]);
-                        du[i] = COMP ? g[i] * left<SIG>(m[r][i]) : g[i];
-                        da[i] = g[i] * h;
-                        if constexpr (SIG) da[i] = da[i] * (kept<SIG>(m[r][i]) * left<SIG>(m[r][i]));
-                        if (r + 1 == n && last && a.dinitial != nullptr) {
-                            reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = kept<SIG>(m[r][i]) * g[i];
+                        if (live) {
+                            store_pack<T, V>(pg, da);
+                            store_pack<T, V>(px, du);
                         }
                     }
-                    store_pack<T, V>(pg, da);
-                    store_pack<T, V>(px, du);
+                    pg += a.wdgate.t;
+                    px += a.wdx.t;
                 }
-                pg += a.wdgate.t;
-                px += a.wdx.t;
-            }
+            };
+            if (n == R && !last) write(std::true_type{});
+            else write(std::false_type{});
             if (alone) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) carry[i] = g[i];
@@ -141,19 +194,19 @@ __global__ void __launch_bounds__(kThreads, kResident<T, V>) backward_kernel(con
     }
 }
 
-template <class T, int V, int R>
+template <class T, int V, int R, int COPY>
 hmc_status launch_backward(hmc_context_t ctx, BackwardArgs &a, int64_t batch, int32_t flags) {
     const Shape shape = plan_launch(batch, a.time, a.channels, V, R);
     a.tiles = shape.tiles;
     a.items = shape.items;
     a.warps_time = shape.warps_time;
-    const char *what = "linear recurrence gradient kernel launch";
-    switch (flags & (HMC_RECURRENCE_SIGMOID | HMC_RECURRENCE_COMPLEMENT)) {
-        case 0: return launch(ctx, backward_kernel<T, V, R, false, false>, shape, a, what);
-        case HMC_RECURRENCE_SIGMOID: return launch(ctx, backward_kernel<T, V, R, true, false>, shape, a, what);
-        case HMC_RECURRENCE_COMPLEMENT: return launch(ctx, backward_kernel<T, V, R, false, true>, shape, a, what);
-        default: return launch(ctx, backward_kernel<T, V, R, true, true>, shape, a, what);
-    }
+    const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
+        static bool raised[kKnownDevices] = {};
+        constexpr int kShared = COPY > 0 ? kWarps * kStages * kStageRows<R, decltype(complement)::value> * Ring<T, V, COPY>::kRow : 0;
+        return launch(ctx, backward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, raised, kShared, shape, a,
+                      "linear recurrence gradient kernel launch");
+    };
+    return dispatch_flags(flags, go);
 }
 
 }  // namespace
@@ -211,12 +264,16 @@ HMC_API hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_t
         a.channels = channels;
         const bool pairs = layer_vectors(dgate, 4) && layer_vectors(dx, 4) && layer_vectors(gate, 4) && layer_vectors(out, 4) &&
                            layer_vectors(dout, 4) && (!complement || layer_vectors(x, 4));
+        const bool wide = layer_vectors(gate, 16) && layer_vectors(out, 16) && layer_vectors(dout, 16) &&
+                          (!complement || layer_vectors(x, 16)) && layer_vectors(dgate, 4) && layer_vectors(dx, 4);
         return dispatch_float(dt, [&](auto tag) -> hmc_status {
             using T = decltype(tag);
+            constexpr int kWord = sizeof(T) == 8 ? 8 : 4, V = sizeof(T) == 2 ? 2 : 1;
             if constexpr (sizeof(T) == 2) {
-                if (pairs) return time == 1 ? launch_backward<T, 2, 1>(ctx, a, batch, flags) : launch_backward<T, 2, 8>(ctx, a, batch, flags);
+                if (!pairs) return time == 1 ? launch_backward<T, 1, 1, 0>(ctx, a, batch, flags) : launch_backward<T, 1, 8, 0>(ctx, a, batch, flags);
             }
-            return time == 1 ? launch_backward<T, 1, 1>(ctx, a, batch, flags) : launch_backward<T, 1, 8>(ctx, a, batch, flags);
+            if (time == 1) return launch_backward<T, V, 1, 0>(ctx, a, batch, flags);
+            return wide ? launch_backward<T, V, 8, 16>(ctx, a, batch, flags) : launch_backward<T, V, 8, kWord>(ctx, a, batch, flags);
         });
     });
 }
