@@ -3,7 +3,7 @@
 // Three steps: every block takes the moments of its run of rows (held in registers: the mean first, then the squares of
 // the deviations from it, run by run merged pairwise), a small kernel merges the pieces of each group, and an elementwise
 // pass normalises. Where one block holds a whole group the middle step falls away.
-#include "group_norm.cuh"
+#include "group_norm_rows.cuh"
 
 namespace hmc {
 namespace gnorm {
@@ -223,8 +223,9 @@ Plan make_plan(const Problem &p, bool vectors) {
 
 // What the forward pass needs whatever the alignment of its operands.
 int64_t forward_workspace(const Problem &p) {
-    const int64_t a = make_plan(p, false).bytes;
-    const int64_t b = p.channels % (16 / element_size(p.dtype)) == 0 ? make_plan(p, true).bytes : 0;
+    const int vector = 16 / element_size(p.dtype);
+    const auto need = [&](bool vectors) -> int64_t { return make_teams(p, vector, vectors, false).v > 0 ? 0 : make_plan(p, vectors).bytes; };
+    const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
     return a > b ? a : b;
 }
 
@@ -259,6 +260,29 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
         if (s != HMC_OK) return s;
         HMC_ENTER(ctx);
         const bool vectors = all_vectors(src, out);
+        const Teams teams = make_teams(p, 16 / element_size(p.dtype), vectors, false);
+        if (teams.v > 0) {
+            RowsForwardArgs r{};
+            r.out = layer_base(out);
+            r.src = layer_base(src);
+            r.wout = Rows{out->strides[0], out->strides[1]};
+            r.wsrc = Rows{src->strides[0], src->strides[1]};
+            r.t = teams;
+            r.samples = p.samples;
+            r.groups = p.groups;
+            r.cg = p.channels / p.groups;
+            r.affine = affine;
+            r.mean = layer_base(mean);
+            r.rstd = layer_base(rstd);
+            if (mean != nullptr) {
+                r.mean_n = mean->strides[0];
+                r.mean_g = mean->strides[1];
+                r.rstd_n = rstd->strides[0];
+                r.rstd_g = rstd->strides[1];
+            }
+            r.eps = eps;
+            return launch_rows_forward(ctx, p.dtype, activation, r);
+        }
         const Plan plan = make_plan(p, vectors);
         StatArgs st{};
         st.src = layer_base(src);

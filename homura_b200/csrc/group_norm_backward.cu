@@ -3,7 +3,7 @@
 // Three steps: sums over each run of rows of dz and dz * xhat (by channel for weight and bias, by group, weighted, for
 // the input), a small kernel that folds the runs in order, and an elementwise pass. Channel sums are kept in f64 across
 // the runs a block takes, and folded over the blocks in f64.
-#include "group_norm.cuh"
+#include "group_norm_rows.cuh"
 
 namespace hmc {
 namespace gnorm {
@@ -23,7 +23,7 @@ struct GradArgs {
     Affine affine;
     void *pieces;         // Two<C> [samples][groups][chunks * segments]
     void *means;          // Two<C> [samples][groups]: the means of p and of p * xhat
-    double *by_channel;   // [columns][2][channels], null when neither dweight nor dbias is wanted
+    void *by_channel;     // [columns][2][channels], f64 (C after the one-pass kernel); null when neither dweight nor dbias is wanted
 };
 
 // One element: xhat and dz, with the forward pass's steps (unfused) up to z.
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kBlock, 2) sums_kernel(const __grid_constant__
         for (int c = threadIdx.x; c < tile.width; c += kBlock) {
             double sum = 0.0;
             for (int y = 0; y < a.t.ty; ++y) sum += shared.by_column[y * tile.width + c];
-            a.by_channel[(column * 2 + which) * a.t.channels + tile.channel + c] = sum;
+            reinterpret_cast<double *>(a.by_channel)[(column * 2 + which) * a.t.channels + tile.channel + c] = sum;
         }
         __syncthreads();
     }
@@ -154,7 +154,7 @@ template <class C> __global__ void __launch_bounds__(kBlock) fold_groups_kernel(
 }
 
 // dweight and dbias: 32 channels a block, eight warps along the blocks that hold partial sums.
-template <class T> __global__ void __launch_bounds__(kBlock) fold_channels_kernel(const __grid_constant__ GradArgs a) {
+template <class T, class P> __global__ void __launch_bounds__(kBlock) fold_channels_kernel(const __grid_constant__ GradArgs a) {
     __shared__ double part[kWarps][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int which = static_cast<int>(blockIdx.x & 1);
@@ -165,7 +165,7 @@ template <class T> __global__ void __launch_bounds__(kBlock) fold_channels_kerne
         const int64_t channel = block * 32 + lane;
         double sum = 0.0;
         if (channel < a.t.channels) {
-            for (int64_t k = warp; k < a.columns; k += kWarps) sum += a.by_channel[(k * 2 + which) * a.t.channels + channel];
+            for (int64_t k = warp; k < a.columns; k += kWarps) sum += static_cast<double>(reinterpret_cast<const P *>(a.by_channel)[(k * 2 + which) * a.t.channels + channel]);
         }
         part[warp][lane] = sum;
         __syncthreads();
@@ -240,11 +240,39 @@ Plan make_plan(const Problem &p, bool vectors) {
     return r;
 }
 
+// The one-pass kernel: at most 64 samples a team (what f32 sums of dz are kept over), fewer where that leaves SMs idle.
+struct RowRuns {
+    Teams t;
+    int64_t run, row_blocks, partials, bytes;
+};
+RowRuns make_runs(const Problem &p, int vector, bool vectors) {
+    RowRuns r{};
+    if (p.positions != 1) return r;
+    r.t = make_teams(p, vector, vectors, true);
+    if (r.t.v == 0) return r;
+    const int64_t rounds = ceil_div(p.samples, r.t.samples_at_once);
+    int64_t run = ceil_div(rounds * r.t.tiles, 148 * 8);
+    run = run < 4 ? 4 : (run > 64 ? 64 : run);
+    if (ceil_div(rounds, run) > 65535 || r.t.tiles > (int64_t{1} << 30)) {  // beyond a grid's second dimension
+        r.t.v = 0;
+        return r;
+    }
+    r.run = run;
+    r.row_blocks = ceil_div(rounds, run);
+    r.partials = r.row_blocks * r.t.samples_at_once;
+    r.bytes = ceil_div(r.partials * 2 * p.channels * element_size(p.stat_dtype), 16) * 16;
+    return r;
+}
+
 }  // namespace
 
 int64_t backward_workspace(const Problem &p) {
-    const int64_t a = make_plan(p, false).bytes;
-    const int64_t b = p.channels % (16 / element_size(p.dtype)) == 0 ? make_plan(p, true).bytes : 0;
+    const int vector = 16 / element_size(p.dtype);
+    const auto need = [&](bool vectors) -> int64_t {
+        const RowRuns r = make_runs(p, vector, vectors);
+        return r.t.v > 0 ? r.bytes : make_plan(p, vectors).bytes;
+    };
+    const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
     return a > b ? a : b;
 }
 int64_t forward_workspace(const Problem &p);
@@ -319,11 +347,13 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
         if (empty) {  // sums over nothing
             a.t.channels = p.channels;
             return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
-                fold_channels_kernel<decltype(tag)><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+                fold_channels_kernel<decltype(tag), double><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
                 return launch_status("group norm channel kernel launch");
             });
         }
-        const Plan plan = make_plan(p, all_vectors(src, dout, dsrc));
+        const bool vectors = all_vectors(src, dout, dsrc);
+        const RowRuns rows = make_runs(p, 16 / element_size(p.dtype), vectors);
+        const Plan plan = rows.t.v > 0 ? Plan{} : make_plan(p, vectors);
         a.src = layer_base(src);
         a.dout = layer_base(dout);
         a.mean = layer_base(mean);
@@ -335,6 +365,39 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
         a.mean_g = mean->strides[1];
         a.rstd_n = rstd->strides[0];
         a.rstd_g = rstd->strides[1];
+        if (rows.t.v > 0) {
+            RowsBackwardArgs b{};
+            b.dsrc = a.dsrc;
+            b.src = a.src;
+            b.dout = a.dout;
+            b.mean = a.mean;
+            b.rstd = a.rstd;
+            b.wdsrc = a.wdsrc;
+            b.wsrc = a.wsrc;
+            b.wdout = a.wdout;
+            b.mean_n = a.mean_n;
+            b.mean_g = a.mean_g;
+            b.rstd_n = a.rstd_n;
+            b.rstd_g = a.rstd_g;
+            b.t = rows.t;
+            b.samples = p.samples;
+            b.groups = p.groups;
+            b.cg = p.channels / p.groups;
+            b.channels = p.channels;
+            b.run = rows.run;
+            b.affine = affine;
+            b.by_channel = sums_wanted ? workspace : nullptr;
+            s = launch_rows_backward(ctx, p.dtype, activation, b, rows.row_blocks);
+            if (s != HMC_OK || !sums_wanted) return s;
+            a.t.channels = p.channels;
+            a.columns = rows.partials;
+            a.by_channel = workspace;
+            return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
+                using T = decltype(tag);
+                fold_channels_kernel<T, typename Comp<T>::C><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+                return launch_status("group norm channel kernel launch");
+            });
+        }
         a.t = plan.t;
         a.cut = plan.sums;
         a.columns = plan.columns;
@@ -342,7 +405,7 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
         a.affine = affine;
         a.pieces = workspace;
         a.means = static_cast<char *>(workspace) + plan.pieces_bytes;
-        a.by_channel = sums_wanted ? reinterpret_cast<double *>(static_cast<char *>(a.means) + plan.means_bytes) : nullptr;
+        a.by_channel = sums_wanted ? static_cast<char *>(a.means) + plan.means_bytes : nullptr;
         return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
             using T = decltype(tag);
             using C = typename Comp<T>::C;
@@ -358,7 +421,7 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
                         l = launch_status("group norm fold kernel launch");
                     }
                     if (l == HMC_OK && sums_wanted) {
-                        fold_channels_kernel<T><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+                        fold_channels_kernel<T, double><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
                         l = launch_status("group norm channel kernel launch");
                     }
                     if (l != HMC_OK) return l;

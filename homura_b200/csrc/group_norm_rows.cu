@@ -1,0 +1,137 @@
+// Group norm with an activation where a group of one sample fits the registers of a team of lanes, forward; the split is
+// group_norm_rows.cuh's.
+#include "group_norm_rows.cuh"
+
+namespace hmc {
+namespace gnorm {
+namespace {
+
+template <class T, int V, int K, bool WIDE, int ACT>
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
+    using C = typename Comp<T>::C;
+    constexpr bool kFast = sizeof(T) == 2;
+    constexpr int U = samples_in_flight(K);
+    constexpr bool kKeep = K * V <= 16;  // parameters in registers
+    __shared__ C scratch[U][kWarps];
+    const int team = threadIdx.x / a.t.lanes, lane = threadIdx.x - team * a.t.lanes;
+    const int beside = team / a.t.groups_per_tile;  // which of the samples side by side
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * a.t.groups_per_tile + (team - beside * a.t.groups_per_tile);
+    const bool team_live = beside < a.t.samples_at_once && group < a.groups;
+    // this lane's vectors: where they lie within a sample, and their channels
+    int64_t in[K], to[K], channel[K];
+    bool have[K];
+    C w[kKeep ? K : 1][V], b[kKeep ? K : 1][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int vector = lane + k * a.t.lanes;
+        have[k] = team_live && vector < a.t.vectors;
+        const int position = vector / a.t.row_vectors;
+        channel[k] = group * a.cg + static_cast<int64_t>(vector - position * a.t.row_vectors) * V;
+        in[k] = position * a.wsrc.s + channel[k];
+        to[k] = position * a.wout.s + channel[k];
+        if constexpr (kKeep) {
+            if (have[k]) {
+                parameters<T, V>(w[k], a.affine.weight, channel[k], a.affine.weight_stride, a.affine.is_f32, C(1));
+                parameters<T, V>(b[k], a.affine.bias, channel[k], a.affine.bias_stride, a.affine.is_f32, C(0));
+            }
+        }
+    }
+    const C count = static_cast<C>(a.t.vectors) * C(V);
+    const int64_t step = static_cast<int64_t>(a.t.samples_at_once) * U;
+    for (int64_t base = blockIdx.y * step; base < a.samples; base += gridDim.y * step) {
+        Pack<T, V> x[U][K];
+        bool live[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t n = base + static_cast<int64_t>(u) * a.t.samples_at_once + beside;
+            live[u] = n < a.samples;
+            const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (live[u] && have[k]) x[u][k] = *reinterpret_cast<const Pack<T, V> *>(src + in[k]);
+                else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[u][k].v[i] = down<T>(C(0));
+                }
+            }
+        }
+        C mean[U], sq[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            mean[u] = C(0);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) mean[u] += up(x[u][k].v[i]);
+            }
+        }
+        team_sum<U, WIDE>(mean, a.t.lanes, scratch);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            mean[u] = mean[u] / count;
+            sq[u] = C(0);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (have[k]) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const C d = up(x[u][k].v[i]) - mean[u];
+                        sq[u] = m_fma(d, d, sq[u]);
+                    }
+                }
+            }
+        }
+        team_sum<U, WIDE>(sq, a.t.lanes, scratch);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t n = base + static_cast<int64_t>(u) * a.t.samples_at_once + beside;
+            const C rstd = C(1) / m_sqrt(sq[u] / count + static_cast<C>(a.eps));
+            if (!live[u]) continue;
+            if (a.mean != nullptr && lane == 0 && team_live) {
+                reinterpret_cast<C *>(a.mean)[n * a.mean_n + group * a.mean_g] = mean[u];
+                reinterpret_cast<C *>(a.rstd)[n * a.rstd_n + group * a.rstd_g] = rstd;
+            }
+            T *out = reinterpret_cast<T *>(a.out) + n * a.wout.n;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (!have[k]) continue;
+                if constexpr (!kKeep) {
+                    parameters<T, V>(w[0], a.affine.weight, channel[k], a.affine.weight_stride, a.affine.is_f32, C(1));
+                    parameters<T, V>(b[0], a.affine.bias, channel[k], a.affine.bias_stride, a.affine.is_f32, C(0));
+                }
+                C y[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    // (the steps of the backward pass, unfused, so that both see the same sign of z)
+                    const C z = (up(x[u][k].v[i]) - mean[u]) * rstd * w[kKeep ? k : 0][i] + b[kKeep ? k : 0][i];
+                    y[i] = activate<ACT, C, kFast>(z);
+                }
+                *reinterpret_cast<Pack<T, V> *>(out + to[k]) = pack_of<T, V>(y);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation, const RowsForwardArgs &a) {
+    return dispatch_float(dtype, [&](auto tag) -> hmc_status {
+        using T = decltype(tag);
+        return dispatch_teams<T, false>(a.t, [&](auto v, auto k, auto wide) -> hmc_status {
+            constexpr int V = decltype(v)::value, K = decltype(k)::value;
+            constexpr bool WIDE = decltype(wide)::value;
+            return dispatch_activation(activation, [&](auto act) -> hmc_status {
+                // about sixteen blocks an SM, each taking several rounds of samples with its parameters in registers
+                const int64_t rounds = ceil_div(a.samples, static_cast<int64_t>(a.t.samples_at_once) * samples_in_flight(K));
+                const int64_t wanted = ceil_div(148 * 16, a.t.tiles);
+                const int64_t y = rounds < wanted ? rounds : wanted;
+                const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(y < 65535 ? y : 65535));
+                rows_kernel<T, V, K, WIDE, decltype(act)::value><<<grid, kBlock, 0, ctx->stream>>>(a);
+                return launch_status("group norm kernel launch");
+            });
+        });
+    });
+}
+
+}  // namespace gnorm
+}  // namespace hmc

@@ -1,0 +1,185 @@
+// Group norm where a group of one sample fits the registers of a team of lanes: every token by itself (one position), or
+// few positions. One pass: a value is read once and written once.
+//
+// A team is a power of two of lanes within a warp (or, WIDE, the whole block); a lane keeps K vectors of V neighbouring
+// channels of its team's group, the same channels for every sample it takes, so parameters (and, backward, the sums for
+// dweight and dbias) stay in registers across samples. U samples are in flight at once, so that a lane has at least four
+// vectors of 16 bytes on their way. Sums go through shuffles within the team.
+#pragma once
+
+#include "group_norm.cuh"
+
+namespace hmc {
+namespace gnorm {
+
+// A lane's vectors at most: 32 values forward, 16 backward, where the sums for dweight and dbias stand beside them.
+constexpr int most_vectors(int v, bool backward) { return (backward ? 16 : 32) / v < 8 ? (backward ? 16 : 32) / v : 8; }
+
+struct Teams {
+    int32_t lanes;            // lanes a team
+    int32_t k;                // vectors a lane
+    int32_t vectors;          // vectors of a group: positions * cg / V
+    int32_t row_vectors;      // cg / V
+    int32_t groups_per_tile;  // groups side by side in a block
+    int32_t samples_at_once;  // samples side by side in a block
+    int64_t tiles;
+    int32_t v;                // 0: the group does not fit
+    bool wide;
+};
+
+// The widest team that wastes least: K * lanes as small as possible, lanes as many as possible for coalescing.
+inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backward) {
+    Teams t{};
+    const int64_t cg = p.channels / p.groups;
+    const int v = vectors && cg % vector == 0 ? vector : 1;
+    const int most_k = most_vectors(v, backward);
+    const int64_t most = static_cast<int64_t>(kBlock) * most_k;
+    if (p.positions > most || cg / v > most || p.positions * (cg / v) > most) return t;
+    t.v = v;
+    t.vectors = static_cast<int32_t>(p.positions * (cg / v));
+    t.row_vectors = static_cast<int32_t>(cg / v);
+    if (t.vectors > 32 * most_k) {
+        t.wide = true;
+        t.lanes = kBlock;
+        t.k = (t.vectors + kBlock - 1) / kBlock;
+    } else {
+        int best = 0;
+        for (int lanes = 32; lanes >= 1; lanes >>= 1) {
+            const int k = (t.vectors + lanes - 1) / lanes;
+            if (k > most_k) break;
+            if (best == 0 || lanes * k < best) {
+                best = lanes * k;
+                t.lanes = lanes;
+                t.k = k;
+            }
+        }
+    }
+    const int64_t teams = kBlock / t.lanes;
+    t.groups_per_tile = static_cast<int32_t>(p.groups < teams ? p.groups : teams);
+    t.samples_at_once = static_cast<int32_t>(teams / t.groups_per_tile);
+    t.tiles = ceil_div(p.groups, t.groups_per_tile);
+    return t;
+}
+constexpr int samples_in_flight(int k) { return k == 1 ? 4 : (k == 2 ? 2 : 1); }
+
+// Sums `s` over the team; every lane gets the same.
+template <int U, bool WIDE, class C> __device__ __forceinline__ void team_sum(C (&s)[U], int lanes, C (*scratch)[kWarps]) {
+    if constexpr (WIDE) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) s[u] += __shfl_xor_sync(0xFFFFFFFFu, s[u], d);
+            if (lane == 0) scratch[u][warp] = s[u];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = scratch[u][0];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) s[u] += scratch[u][w];
+        }
+        __syncthreads();
+    } else {
+        for (int d = lanes >> 1; d > 0; d >>= 1) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] += __shfl_xor_sync(0xFFFFFFFFu, s[u], d);
+        }
+    }
+}
+
+// V parameters from channel `at` on, or `otherwise` where there are none.
+template <class T, int V> __device__ __forceinline__ void parameters(typename Comp<T>::C (&to)[V], const char *p, int64_t at, int64_t stride,
+                                                                     int is_f32, typename Comp<T>::C otherwise) {
+    using C = typename Comp<T>::C;
+    if (p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = otherwise;
+        return;
+    }
+    if constexpr (V > 1) {
+        if (stride == 1 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {  // (at is a multiple of V)
+            if (is_f32) {
+                constexpr int kHalf = V < 4 ? V : 4;
+#pragma unroll
+                for (int h = 0; h < V; h += kHalf) {
+                    const Pack<float, kHalf> w = *reinterpret_cast<const Pack<float, kHalf> *>(reinterpret_cast<const float *>(p) + at + h);
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) to[h + i] = static_cast<C>(w.v[i]);
+                }
+            } else {
+                const Pack<T, V> w = *reinterpret_cast<const Pack<T, V> *>(reinterpret_cast<const T *>(p) + at);
+#pragma unroll
+                for (int i = 0; i < V; ++i) to[i] = up(w.v[i]);
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[i] = parameter<T>(p, (at + i) * stride, is_f32);
+}
+
+template <class T, int V> __device__ __forceinline__ Pack<T, V> pack_of(const typename Comp<T>::C (&v)[V]) {
+    Pack<T, V> r;
+    if constexpr (V % 2 == 0 && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) down2(r.v[i], r.v[i + 1], v[i], v[i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = down<T>(v[i]);
+    }
+    return r;
+}
+
+struct RowsForwardArgs {
+    char *out;
+    const char *src;
+    Rows wout, wsrc;
+    Teams t;
+    int64_t samples, groups, cg;
+    Affine affine;
+    char *mean, *rstd;  // or null
+    int64_t mean_n, mean_g, rstd_n, rstd_g;
+    double eps;
+};
+struct RowsBackwardArgs {
+    char *dsrc;
+    const char *src, *dout, *mean, *rstd;
+    Rows wdsrc, wsrc, wdout;
+    int64_t mean_n, mean_g, rstd_n, rstd_g;
+    Teams t;
+    int64_t samples, groups, cg, channels;
+    int64_t run;        // samples a team takes
+    Affine affine;
+    void *by_channel;   // C [row blocks * samples_at_once][2][channels], or null
+};
+
+// One launch; the group of a sample fits a team (t.v > 0). dispatch.
+hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation, const RowsForwardArgs &a);
+// positions == 1
+hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation, const RowsBackwardArgs &a, int64_t row_blocks);
+
+// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (8 only without vectors, 2 at least for a block).
+template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(const Teams &t, F &&f) {
+    constexpr int V = kVector<T>, kMost = most_vectors(V, BACKWARD);
+    const auto with = [&](auto v, auto k, auto wide) { return f(v, k, wide); };
+    using One = std::integral_constant<int, 1>;
+    using Vec = std::integral_constant<int, V>;
+    if (t.v == 1) {
+        if (t.wide) return with(One{}, std::integral_constant<int, 8>{}, std::true_type{});
+        return with(One{}, std::integral_constant<int, 8>{}, std::false_type{});
+    }
+    if (t.wide) {
+        if (t.k <= 2) return with(Vec{}, std::integral_constant<int, 2>{}, std::true_type{});
+        return with(Vec{}, std::integral_constant<int, kMost>{}, std::true_type{});
+    }
+    if (t.k <= 1) return with(Vec{}, One{}, std::false_type{});
+    if (t.k <= 2) return with(Vec{}, std::integral_constant<int, 2>{}, std::false_type{});
+    if constexpr (kMost >= 4) {
+        if (t.k <= 4) return with(Vec{}, std::integral_constant<int, 4>{}, std::false_type{});
+    }
+    return with(Vec{}, std::integral_constant<int, kMost>{}, std::false_type{});
+}
+
+}  // namespace gnorm
+}  // namespace hmc

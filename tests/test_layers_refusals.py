@@ -85,8 +85,10 @@ def test_recurrence_backward_refusals():
 def test_group_norm_refusals():
     lib = homura_b200.load()
     t, stat, par = desc([2, 3, 8]), desc([2, 4]), desc([8])
+    long = desc([2, 100000, 8])  # a group that no block holds: its pieces' moments need a workspace
     nbytes = ctypes.c_int64(-1)
-    assert lib.hmc_group_norm_workspace(t, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value > 0
+    assert lib.hmc_group_norm_workspace(t, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value >= 0
+    assert lib.hmc_group_norm_workspace(long, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value > 0
     need = nbytes.value
     ws = (HOST.ctypes.data + 15) // 16 * 16
 
@@ -94,11 +96,10 @@ def test_group_norm_refusals():
         return lib.hmc_group_norm(None, out, src, weight, bias, mean, rstd, groups, eps, act, ws, n)
 
     refused(call(), "null context")
-    refused(call(n=need), "null context")
-    if need:
-        refused(call(n=need - 1), f"group norm needs {need}")
-        refused(call(ws=None), f"group norm needs {need}")
-        refused(call(ws=ws + 4), "16-byte aligned")
+    refused(call(out=long, src=long, n=need), "null context")
+    refused(call(out=long, src=long, n=need - 1), f"group norm needs {need}")
+    refused(call(out=long, src=long, ws=None), f"group norm needs {need}")
+    refused(call(out=long, src=long, ws=ws + 4, n=need), "16-byte aligned")
     refused(call(groups=3), "do not divide")
     refused(call(groups=0), "do not divide")
     refused(call(groups=-4), "do not divide")
@@ -125,7 +126,7 @@ def test_group_norm_refusals():
     assert lib.hmc_group_norm_workspace(None, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     assert lib.hmc_group_norm_workspace(t, 5, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     # sizes alone decide: a description without memory is enough
-    assert lib.hmc_group_norm_workspace(desc([2, 3, 8], data=False), 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value == need
+    assert lib.hmc_group_norm_workspace(desc([2, 100000, 8], data=False), 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value == need
 
 
 def test_group_norm_backward_refusals():
