@@ -167,7 +167,6 @@ struct ApplyArgs {
 template <class T, int V, int ACT>
 __global__ void __launch_bounds__(kBlock) apply_kernel(const __grid_constant__ ApplyArgs a) {
     using C = typename Comp<T>::C;
-    constexpr bool kFast = sizeof(T) == 2;
     const int tx = threadIdx.x % a.t.tx, ty = threadIdx.x / a.t.tx;
     for (int64_t unit = blockIdx.x; unit < a.cut.units; unit += gridDim.x) {
         const int64_t strip = unit / a.cut.chunks, chunk = unit - strip * a.cut.chunks;
@@ -194,9 +193,7 @@ __global__ void __launch_bounds__(kBlock) apply_kernel(const __grid_constant__ A
             Pack<T, V> y;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                // (the steps of the backward pass, unfused, so that both see the same sign of z)
-                const C z = (up(x.v[i]) - mean[i]) * rstd[i] * w[i] + b[i];
-                y.v[i] = down<T>(activate<ACT, C, kFast>(z));
+                y.v[i] = down<T>(activate<ACT>(scaled<ACT>((up(x.v[i]) - mean[i]) * rstd[i], w[i], b[i])));
             }
             *reinterpret_cast<Pack<T, V> *>(out + row * a.wout.s) = y;
         }

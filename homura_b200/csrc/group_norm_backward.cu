@@ -26,12 +26,11 @@ struct GradArgs {
     void *by_channel;     // [columns][2][channels], f64 (C after the one-pass kernel); null when neither dweight nor dbias is wanted
 };
 
-// One element: xhat and dz, with the forward pass's steps (unfused) up to z.
-template <class T, int ACT, class C>
+// One element: xhat and dz, with the forward pass's steps up to z.
+template <int ACT, class C>
 __device__ __forceinline__ void element(C x, C dy, C mean, C rstd, C w, C b, C &xhat, C &dz) {
     xhat = (x - mean) * rstd;
-    const C z = xhat * w + b;
-    dz = through<ACT, C, sizeof(T) == 2>(dy, z);
+    dz = through<ACT>(dy, scaled<ACT>(xhat, w, b));
 }
 
 template <class T, int V> struct Coefficients {
@@ -94,7 +93,7 @@ __global__ void __launch_bounds__(kBlock, 2) sums_kernel(const __grid_constant__
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     C xhat, dz;
-                    element<T, ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
+                    element<ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
                     s1[i] += dz;
                     s2[i] = m_fma(dz, xhat, s2[i]);
                 }
@@ -211,7 +210,7 @@ __global__ void __launch_bounds__(kBlock) grad_kernel(const __grid_constant__ Gr
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 C xhat, dz;
-                element<T, ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
+                element<ACT>(up(x.v[i]), up(d.v[i]), k.mean[i], k.rstd[i], k.w[i], k.b[i], xhat, dz);
                 y.v[i] = down<T>(k.rstd[i] * (dz * k.w[i] - m1[i] - xhat * m2[i]));
             }
             *reinterpret_cast<Pack<T, V> *>(dsrc + row * a.wdsrc.s) = y;

@@ -7,10 +7,9 @@ namespace gnorm {
 namespace {
 
 template <class T, int V, int K, bool WIDE, int ACT>
-__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : (V > 1 && K * V <= 8 ? 3 : 2)) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
     using C = typename Comp<T>::C;
-    constexpr bool kFast = sizeof(T) == 2;
-    constexpr int U = samples_in_flight(K);
+    constexpr int U = samples_at_a_time(K);
     constexpr bool kKeep = K * V <= 16;  // parameters in registers
     __shared__ C scratch[U][kWarps];
     const int team = threadIdx.x / a.t.lanes, lane = threadIdx.x - team * a.t.lanes;
@@ -36,25 +35,38 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_kernel(co
             }
         }
     }
-    const C count = static_cast<C>(a.t.vectors) * C(V);
-    const int64_t step = static_cast<int64_t>(a.t.samples_at_once) * U;
-    for (int64_t base = blockIdx.y * step; base < a.samples; base += gridDim.y * step) {
-        Pack<T, V> x[U][K];
-        bool live[U];
+    const C share = C(1) / (static_cast<C>(a.t.vectors) * C(V));
+    const int64_t step = static_cast<int64_t>(a.t.samples_at_once) * U * gridDim.y;
+    const int64_t first = static_cast<int64_t>(blockIdx.y) * a.t.samples_at_once * U;
+    int64_t n = first + beside;  // of the samples at a time, samples_at_once apart, the first
+    const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n;
+    T *out = reinterpret_cast<T *>(a.out) + n * a.wout.n;
+    const int64_t src_next = a.t.samples_at_once * a.wsrc.n, out_next = a.t.samples_at_once * a.wout.n;
+    Pack<T, V> ahead[U][K];
+    const auto load = [&](int64_t from, const T *p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t n = base + static_cast<int64_t>(u) * a.t.samples_at_once + beside;
-            live[u] = n < a.samples;
-            const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (live[u] && have[k]) x[u][k] = *reinterpret_cast<const Pack<T, V> *>(src + in[k]);
-                else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[u][k].v[i] = down<T>(C(0));
-                }
+                if (have[k] && from + u * a.t.samples_at_once < a.samples) ahead[u][k] = *reinterpret_cast<const Pack<T, V> *>(p + u * src_next + in[k]);
             }
         }
+    };
+    load(n, src);
+    // (the loop runs alike for the whole block: the shuffles and barriers of a team's sums stand in it. Lanes without a
+    // vector, or without a sample, add nothing and write nothing.)
+    for (int64_t base = first; base < a.samples; base += step, n += step) {
+        C x[U][K][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[u][k][i] = have[k] ? up(ahead[u][k].v[i]) : C(0);
+            }
+        }
+        src += step * a.wsrc.n;
+        load(n + step, src);
         C mean[U], sq[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -62,36 +74,32 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_kernel(co
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) mean[u] += up(x[u][k].v[i]);
+                for (int i = 0; i < V; ++i) mean[u] += x[u][k][i];
             }
         }
         team_sum<U, WIDE>(mean, a.t.lanes, scratch);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            mean[u] = mean[u] / count;
+            mean[u] *= share;
             sq[u] = C(0);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (have[k]) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const C d = up(x[u][k].v[i]) - mean[u];
-                        sq[u] = m_fma(d, d, sq[u]);
-                    }
+                for (int i = 0; i < V; ++i) {
+                    x[u][k][i] = have[k] ? x[u][k][i] - mean[u] : C(0);
+                    sq[u] = m_fma(x[u][k][i], x[u][k][i], sq[u]);
                 }
             }
         }
         team_sum<U, WIDE>(sq, a.t.lanes, scratch);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t n = base + static_cast<int64_t>(u) * a.t.samples_at_once + beside;
-            const C rstd = C(1) / m_sqrt(sq[u] / count + static_cast<C>(a.eps));
-            if (!live[u]) continue;
+            const C rstd = inverse_root(m_fma(sq[u], share, static_cast<C>(a.eps)));
+            if (n + u * a.t.samples_at_once >= a.samples) continue;
             if (a.mean != nullptr && lane == 0 && team_live) {
-                reinterpret_cast<C *>(a.mean)[n * a.mean_n + group * a.mean_g] = mean[u];
-                reinterpret_cast<C *>(a.rstd)[n * a.rstd_n + group * a.rstd_g] = rstd;
+                reinterpret_cast<C *>(a.mean)[(n + u * a.t.samples_at_once) * a.mean_n + group * a.mean_g] = mean[u];
+                reinterpret_cast<C *>(a.rstd)[(n + u * a.t.samples_at_once) * a.rstd_n + group * a.rstd_g] = rstd;
             }
-            T *out = reinterpret_cast<T *>(a.out) + n * a.wout.n;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (!have[k]) continue;
@@ -101,14 +109,11 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_kernel(co
                 }
                 C y[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    // (the steps of the backward pass, unfused, so that both see the same sign of z)
-                    const C z = (up(x[u][k].v[i]) - mean[u]) * rstd * w[kKeep ? k : 0][i] + b[kKeep ? k : 0][i];
-                    y[i] = activate<ACT, C, kFast>(z);
-                }
-                *reinterpret_cast<Pack<T, V> *>(out + to[k]) = pack_of<T, V>(y);
+                for (int i = 0; i < V; ++i) y[i] = activate<ACT>(scaled<ACT>(x[u][k][i] * rstd, w[kKeep ? k : 0][i], b[kKeep ? k : 0][i]));
+                *reinterpret_cast<Pack<T, V> *>(out + u * out_next + to[k]) = pack_of<T, V>(y);
             }
         }
+        out += step * a.wout.n;
     }
 }
 
@@ -122,7 +127,7 @@ hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation,
             constexpr bool WIDE = decltype(wide)::value;
             return dispatch_activation(activation, [&](auto act) -> hmc_status {
                 // about sixteen blocks an SM, each taking several rounds of samples with its parameters in registers
-                const int64_t rounds = ceil_div(a.samples, static_cast<int64_t>(a.t.samples_at_once) * samples_in_flight(K));
+                const int64_t rounds = ceil_div(a.samples, static_cast<int64_t>(a.t.samples_at_once) * samples_at_a_time(K));
                 const int64_t wanted = ceil_div(148 * 16, a.t.tiles);
                 const int64_t y = rounds < wanted ? rounds : wanted;
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(y < 65535 ? y : 65535));

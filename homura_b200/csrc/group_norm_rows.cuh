@@ -3,8 +3,7 @@
 //
 // A team is a power of two of lanes within a warp (or, WIDE, the whole block); a lane keeps K vectors of V neighbouring
 // channels of its team's group, the same channels for every sample it takes, so parameters (and, backward, the sums for
-// dweight and dbias) stay in registers across samples. U samples are in flight at once, so that a lane has at least four
-// vectors of 16 bytes on their way. Sums go through shuffles within the team.
+// dweight and dbias) stay in registers across samples. The next samples' vectors are loaded while the present ones are worked on. Sums go through shuffles within the team.
 #pragma once
 
 #include "group_norm.cuh"
@@ -60,7 +59,8 @@ inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backwar
     t.tiles = ceil_div(p.groups, t.groups_per_tile);
     return t;
 }
-constexpr int samples_in_flight(int k) { return k == 1 ? 4 : (k == 2 ? 2 : 1); }
+// Samples a lane takes at once; the next ones are on their way meanwhile.
+constexpr int samples_at_a_time(int k) { return k == 1 ? 2 : 1; }
 
 // Sums `s` over the team; every lane gets the same.
 template <int U, bool WIDE, class C> __device__ __forceinline__ void team_sum(C (&s)[U], int lanes, C (*scratch)[kWarps]) {
