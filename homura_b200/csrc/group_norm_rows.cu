@@ -12,6 +12,9 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : (V > 1 && K * V <
     constexpr int U = samples_at_a_time(K);
     constexpr bool kKeep = K * V <= 16;  // parameters in registers
     __shared__ C scratch[U][kWarps];
+    extern __shared__ __align__(16) unsigned char memory[];
+    using Ring = RowRing<T, V, U * K>;
+    Ring ring(memory);
     const int team = threadIdx.x / a.t.lanes, lane = threadIdx.x - team * a.t.lanes;
     const int beside = team / a.t.groups_per_tile;  // which of the samples side by side
     const int64_t group = static_cast<int64_t>(blockIdx.x) * a.t.groups_per_tile + (team - beside * a.t.groups_per_tile);
@@ -42,31 +45,41 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : (V > 1 && K * V <
     const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n;
     T *out = reinterpret_cast<T *>(a.out) + n * a.wout.n;
     const int64_t src_next = a.t.samples_at_once * a.wsrc.n, out_next = a.t.samples_at_once * a.wout.n;
-    Pack<T, V> ahead[U][K];
-    const auto load = [&](int64_t from, const T *p) {
+    const auto load = [&](int64_t from, int stage) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                if (have[k] && from + u * a.t.samples_at_once < a.samples) ahead[u][k] = *reinterpret_cast<const Pack<T, V> *>(p + u * src_next + in[k]);
+                if (have[k] && from + u * a.t.samples_at_once < a.samples) ring.fetch(stage, u * K + k, src + u * src_next + in[k]);
             }
         }
+        ring.commit();
+        src += step * a.wsrc.n;
     };
-    load(n, src);
+    // rounds on their way: all stages but the one being worked on, or the next in registers
+    constexpr int kAhead = Ring::kUsed ? Ring::kStages - 1 : 1;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) load(n + s * step, s);
+    int stage = 0;
     // (the loop runs alike for the whole block: the shuffles and barriers of a team's sums stand in it. Lanes without a
     // vector, or without a sample, add nothing and write nothing.)
     for (int64_t base = first; base < a.samples; base += step, n += step) {
         C x[U][K][V];
+        if constexpr (Ring::kUsed) {
+            load(n + kAhead * step, stage == 0 ? Ring::kStages - 1 : stage - 1);
+            ring.wait();
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                const Pack<T, V> v = ring.get(stage, u * K + k);
 #pragma unroll
-                for (int i = 0; i < V; ++i) x[u][k][i] = have[k] ? up(ahead[u][k].v[i]) : C(0);
+                for (int i = 0; i < V; ++i) x[u][k][i] = have[k] ? up(v.v[i]) : C(0);
             }
         }
-        src += step * a.wsrc.n;
-        load(n + step, src);
+        if constexpr (Ring::kUsed) stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+        else load(n + step, 0);
         C mean[U], sq[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -131,7 +144,12 @@ hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation,
                 const int64_t wanted = ceil_div(148 * 16, a.t.tiles);
                 const int64_t y = rounds < wanted ? rounds : wanted;
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(y < 65535 ? y : 65535));
-                rows_kernel<T, V, K, WIDE, decltype(act)::value><<<grid, kBlock, 0, ctx->stream>>>(a);
+                constexpr int kShared = RowRing<T, V, samples_at_a_time(K) * K>::kBytes;
+                static bool raised[kRowDevices] = {};
+                const auto kernel = rows_kernel<T, V, K, WIDE, decltype(act)::value>;
+                const hmc_status s = raise_shared(ctx, kernel, raised, kShared);
+                if (s != HMC_OK) return s;
+                kernel<<<grid, kBlock, kShared, ctx->stream>>>(a);
                 return launch_status("group norm kernel launch");
             });
         });

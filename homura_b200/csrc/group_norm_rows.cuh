@@ -3,7 +3,9 @@
 //
 // A team is a power of two of lanes within a warp (or, WIDE, the whole block); a lane keeps K vectors of V neighbouring
 // channels of its team's group, the same channels for every sample it takes, so parameters (and, backward, the sums for
-// dweight and dbias) stay in registers across samples. The next samples' vectors are loaded while the present ones are worked on. Sums go through shuffles within the team.
+// dweight and dbias) stay in registers across samples. The next samples' vectors come through a ring in shared
+// memory that a lane's own asynchronous copies of 16 bytes fill rounds ahead (a lane reads only what it copied: waiting for
+// its copies is all the synchronisation); values without vectors are loaded to registers a round ahead. Sums go through shuffles within the team.
 #pragma once
 
 #include "group_norm.cuh"
@@ -59,7 +61,7 @@ inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backwar
     t.tiles = ceil_div(p.groups, t.groups_per_tile);
     return t;
 }
-// Samples a lane takes at once; the next ones are on their way meanwhile.
+// Samples a lane takes at once.
 constexpr int samples_at_a_time(int k) { return k == 1 ? 2 : 1; }
 
 // Sums `s` over the team; every lane gets the same.
@@ -129,6 +131,48 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> pack_of(const ty
         for (int i = 0; i < V; ++i) r.v[i] = down<T>(v[i]);
     }
     return r;
+}
+
+// `WORDS` vectors a lane and round.
+template <class T, int V, int WORDS> struct RowRing {
+    static constexpr bool kUsed = static_cast<int>(sizeof(T)) * V == 16;
+    static constexpr int kRound = WORDS * kBlock * 16;  // bytes a block and round
+    static constexpr int kStages = !kUsed ? 1 : (kRound * 4 <= 49152 ? 4 : (kRound * 3 <= 49152 ? 3 : 2));
+    static constexpr int kBytes = kUsed ? kStages * kRound : 0;
+    Pack<T, V> direct[kUsed ? 1 : WORDS];
+    unsigned char *mine;
+    __device__ __forceinline__ explicit RowRing(unsigned char *memory) : mine(memory + threadIdx.x * 16) {}
+    __device__ __forceinline__ void fetch(int stage, int word, const T *p) {
+        if constexpr (kUsed) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine + (stage * WORDS + word) * (kBlock * 16)))), "l"(p)
+                         : "memory");
+        } else {
+            direct[word] = *reinterpret_cast<const Pack<T, V> *>(p);
+        }
+    }
+    // After the copies of a round; then, before the first read of the oldest round in flight.
+    __device__ __forceinline__ void commit() const {
+        if constexpr (kUsed) async_copy_commit();
+    }
+    __device__ __forceinline__ void wait() const {
+        if constexpr (kUsed) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    }
+    __device__ __forceinline__ Pack<T, V> get(int stage, int word) const {
+        if constexpr (kUsed) return *reinterpret_cast<const Pack<T, V> *>(mine + (stage * WORDS + word) * (kBlock * 16));
+        else return direct[word];
+    }
+};
+
+constexpr int kRowDevices = 64;
+// `raised` remembers, per kernel and device, that the kernel may use its dynamic shared memory (with the static part it
+// may pass 48 KB; a race
+// between threads only repeats the call).
+template <class Kernel> inline hmc_status raise_shared(hmc_context_t ctx, Kernel kernel, bool (&raised)[kRowDevices], int bytes) {
+    if (bytes > 32768 && (ctx->device >= kRowDevices || !raised[ctx->device])) {
+        HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory size of a group norm kernel");
+        if (ctx->device < kRowDevices) raised[ctx->device] = true;
+    }
+    return HMC_OK;
 }
 
 struct RowsForwardArgs {

@@ -12,6 +12,9 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
     using C = typename Comp<T>::C;
     constexpr bool kKeep = K * V <= 8;  // parameters in registers
     __shared__ C scratch[2][kWarps];
+    extern __shared__ __align__(16) unsigned char memory[];
+    using Ring = RowRing<T, V, 2 * K>;  // src, then dout
+    Ring ring(memory);
     const int team = threadIdx.x / a.t.lanes, lane = threadIdx.x - team * a.t.lanes;
     const int beside = team / a.t.groups_per_tile;
     const int64_t group = static_cast<int64_t>(blockIdx.x) * a.t.groups_per_tile + (team - beside * a.t.groups_per_tile);
@@ -39,25 +42,42 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
     const T *dout = reinterpret_cast<const T *>(a.dout) + n * a.wdout.n + first_channel + at;
     T *dsrc = reinterpret_cast<T *>(a.dsrc) + n * a.wdsrc.n + first_channel + at;
     const int64_t src_next = a.t.samples_at_once * a.wsrc.n, dout_next = a.t.samples_at_once * a.wdout.n, dsrc_next = a.t.samples_at_once * a.wdsrc.n;
-    Pack<T, V> x_ahead[K], d_ahead[K];
-    C mean_ahead = C(0), rstd_ahead = C(0);
-    const auto load = [&](int64_t sample, int64_t r) {
-        if (r >= a.run || sample >= a.samples || !team_live) return;
-        mean_ahead = reinterpret_cast<const C *>(a.mean)[sample * a.mean_n + group * a.mean_g];
-        rstd_ahead = reinterpret_cast<const C *>(a.rstd)[sample * a.rstd_n + group * a.rstd_g];
+    const auto load = [&](int64_t sample, int64_t r, int stage) {
+        if (r < a.run && sample < a.samples) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            if (have[k]) {
-                x_ahead[k] = *reinterpret_cast<const Pack<T, V> *>(src + k * apart);
-                d_ahead[k] = *reinterpret_cast<const Pack<T, V> *>(dout + k * apart);
+            for (int k = 0; k < K; ++k) {
+                if (have[k]) {
+                    ring.fetch(stage, k, src + k * apart);
+                    ring.fetch(stage, K + k, dout + k * apart);
+                }
             }
         }
+        ring.commit();
+        src += src_next;
+        dout += dout_next;
     };
-    load(n, 0);
+    // rounds on their way: all stages but the one being worked on, or the next in registers
+    constexpr int kAhead = Ring::kUsed ? Ring::kStages - 1 : 1;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) load(n + s * a.t.samples_at_once, s, s);
+    C mean_ahead = C(0), rstd_ahead = C(0);
+    const auto load_moments = [&](int64_t sample) {
+        if (sample < a.samples && team_live) {
+            mean_ahead = reinterpret_cast<const C *>(a.mean)[sample * a.mean_n + group * a.mean_g];
+            rstd_ahead = reinterpret_cast<const C *>(a.rstd)[sample * a.rstd_n + group * a.rstd_g];
+        }
+    };
+    load_moments(n);
+    int stage = 0;
     // (the loop runs alike for the whole block: the shuffles and barriers of a team's sums stand in it)
     for (int64_t r = 0; r < a.run && first + r * a.t.samples_at_once < a.samples; ++r, n += a.t.samples_at_once) {
         const bool live = n < a.samples && team_live;
         const C mean = mean_ahead, rstd = rstd_ahead;
+        load_moments(n + a.t.samples_at_once);
+        if constexpr (Ring::kUsed) {
+            load(n + kAhead * a.t.samples_at_once, r + kAhead, stage == 0 ? Ring::kStages - 1 : stage - 1);
+            ring.wait();
+        }
         C xhat[K][V], p[K][V], sums[2] = {C(0), C(0)};  // of p and of p * xhat
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -68,10 +88,11 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
                 }
             }
             if (!live || !have[k]) continue;
+            const Pack<T, V> x = ring.get(stage, k), d = ring.get(stage, K + k);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                xhat[k][i] = (up(x_ahead[k].v[i]) - mean) * rstd;
-                const C g = through<ACT>(up(d_ahead[k].v[i]), scaled<ACT>(xhat[k][i], w[kKeep ? k : 0][i], b[kKeep ? k : 0][i]));
+                xhat[k][i] = (up(x.v[i]) - mean) * rstd;
+                const C g = through<ACT>(up(d.v[i]), scaled<ACT>(xhat[k][i], w[kKeep ? k : 0][i], b[kKeep ? k : 0][i]));
                 dw[k][i] = m_fma(g, xhat[k][i], dw[k][i]);
                 db[k][i] += g;
                 p[k][i] = g * w[kKeep ? k : 0][i];
@@ -79,9 +100,8 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
                 sums[1] = m_fma(p[k][i], xhat[k][i], sums[1]);
             }
         }
-        src += src_next;
-        dout += dout_next;
-        load(n + a.t.samples_at_once, r + 1);
+        if constexpr (Ring::kUsed) stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+        else load(n + a.t.samples_at_once, r + 1, 0);
         team_sum<2, WIDE>(sums, a.t.lanes, scratch);
         const C m1 = sums[0] * share, m2 = sums[1] * share;
 #pragma unroll
@@ -117,7 +137,12 @@ hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation
             constexpr bool WIDE = decltype(wide)::value;
             return dispatch_activation(activation, [&](auto act) -> hmc_status {
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(row_blocks));
-                rows_backward_kernel<T, V, K, WIDE, decltype(act)::value><<<grid, kBlock, 0, ctx->stream>>>(a);
+                constexpr int kShared = RowRing<T, V, 2 * K>::kBytes;
+                static bool raised[kRowDevices] = {};
+                const auto kernel = rows_backward_kernel<T, V, K, WIDE, decltype(act)::value>;
+                const hmc_status s = raise_shared(ctx, kernel, raised, kShared);
+                if (s != HMC_OK) return s;
+                kernel<<<grid, kBlock, kShared, ctx->stream>>>(a);
                 return launch_status("group norm gradient kernel launch");
             });
         });
