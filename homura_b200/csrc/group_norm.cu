@@ -3,7 +3,7 @@
 // Three steps: every block takes the moments of its run of rows (held in registers: the mean first, then the squares of
 // the deviations from it, run by run merged pairwise), a small kernel merges the pieces of each group, and an elementwise
 // pass normalises. Where one block holds a whole group the middle step falls away.
-#include "group_norm_rows.cuh"
+#include "group_norm_resident.cuh"
 
 namespace hmc {
 namespace gnorm {
@@ -221,7 +221,10 @@ Plan make_plan(const Problem &p, bool vectors) {
 // What the forward pass needs whatever the alignment of its operands.
 int64_t forward_workspace(const Problem &p) {
     const int vector = 16 / element_size(p.dtype);
-    const auto need = [&](bool vectors) -> int64_t { return make_teams(p, vector, vectors, false).v > 0 ? 0 : make_plan(p, vectors).bytes; };
+    const auto need = [&](bool vectors) -> int64_t {
+        if (make_teams(p, vector, vectors, false).v > 0 || make_resident(p, vector, vectors, 1).t.v > 0) return 0;
+        return make_plan(p, vectors).bytes;
+    };
     const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
     return a > b ? a : b;
 }
@@ -279,6 +282,28 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
             }
             r.eps = eps;
             return launch_rows_forward(ctx, p.dtype, activation, r);
+        }
+        const Resident resident = make_resident(p, 16 / element_size(p.dtype), vectors, 1);
+        if (resident.t.v > 0) {
+            ResidentForwardArgs r{};
+            r.out = layer_base(out);
+            r.src = layer_base(src);
+            r.wout = Rows{out->strides[0], out->strides[1]};
+            r.wsrc = Rows{src->strides[0], src->strides[1]};
+            r.r = resident;
+            r.samples = p.samples;
+            r.positions = p.positions;
+            r.affine = affine;
+            r.mean = layer_base(mean);
+            r.rstd = layer_base(rstd);
+            if (mean != nullptr) {
+                r.mean_n = mean->strides[0];
+                r.mean_g = mean->strides[1];
+                r.rstd_n = rstd->strides[0];
+                r.rstd_g = rstd->strides[1];
+            }
+            r.eps = eps;
+            return launch_resident_forward(ctx, p.dtype, activation, r);
         }
         const Plan plan = make_plan(p, vectors);
         StatArgs st{};

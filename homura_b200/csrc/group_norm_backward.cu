@@ -3,7 +3,7 @@
 // Three steps: sums over each run of rows of dz and dz * xhat (by channel for weight and bias, by group, weighted, for
 // the input), a small kernel that folds the runs in order, and an elementwise pass. Channel sums are kept in f64 across
 // the runs a block takes, and folded over the blocks in f64.
-#include "group_norm_rows.cuh"
+#include "group_norm_resident.cuh"
 
 namespace hmc {
 namespace gnorm {
@@ -263,13 +263,23 @@ RowRuns make_runs(const Problem &p, int vector, bool vectors) {
     return r;
 }
 
+// Clusters that share a tile of the resident kernel.
+int64_t resident_columns(const Problem &p, const Resident &r) {
+    int64_t wanted = ceil_div(kBlocksWanted, r.t.tiles * r.cluster);
+    const int64_t least = ceil_div(p.samples, 64);  // samples whose sums one block keeps in the computation type
+    if (wanted < least) wanted = least;
+    return wanted < p.samples ? wanted : p.samples;
+}
+
 }  // namespace
 
 int64_t backward_workspace(const Problem &p) {
     const int vector = 16 / element_size(p.dtype);
     const auto need = [&](bool vectors) -> int64_t {
         const RowRuns r = make_runs(p, vector, vectors);
-        return r.t.v > 0 ? r.bytes : make_plan(p, vectors).bytes;
+        if (r.t.v > 0) return r.bytes;
+        const Resident resident = make_resident(p, vector, vectors, 2);
+        return resident.t.v > 0 ? ceil_div(resident_columns(p, resident) * resident.cluster * 2 * p.channels * element_size(p.stat_dtype), 16) * 16 : make_plan(p, vectors).bytes;
     };
     const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
     return a > b ? a : b;
@@ -352,7 +362,8 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
         }
         const bool vectors = all_vectors(src, dout, dsrc);
         const RowRuns rows = make_runs(p, 16 / element_size(p.dtype), vectors);
-        const Plan plan = rows.t.v > 0 ? Plan{} : make_plan(p, vectors);
+        const Resident resident = rows.t.v > 0 ? Resident{} : make_resident(p, 16 / element_size(p.dtype), vectors, 2);
+        const Plan plan = rows.t.v > 0 || resident.t.v > 0 ? Plan{} : make_plan(p, vectors);
         a.src = layer_base(src);
         a.dout = layer_base(dout);
         a.mean = layer_base(mean);
@@ -364,6 +375,14 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
         a.mean_g = mean->strides[1];
         a.rstd_n = rstd->strides[0];
         a.rstd_g = rstd->strides[1];
+        const auto fold_by_channel = [&](int64_t partials, auto tag) -> hmc_status {
+            a.t.channels = p.channels;
+            a.columns = partials;
+            a.by_channel = workspace;
+            using T = decltype(tag);
+            fold_channels_kernel<T, typename Comp<T>::C><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
+            return launch_status("group norm channel kernel launch");
+        };
         if (rows.t.v > 0) {
             RowsBackwardArgs b{};
             b.dsrc = a.dsrc;
@@ -388,14 +407,31 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
             b.by_channel = sums_wanted ? workspace : nullptr;
             s = launch_rows_backward(ctx, p.dtype, activation, b, rows.row_blocks);
             if (s != HMC_OK || !sums_wanted) return s;
-            a.t.channels = p.channels;
-            a.columns = rows.partials;
-            a.by_channel = workspace;
-            return dispatch_float(p.dtype, [&](auto tag) -> hmc_status {
-                using T = decltype(tag);
-                fold_channels_kernel<T, typename Comp<T>::C><<<grid_for(channel_blocks), kBlock, 0, ctx->stream>>>(a);
-                return launch_status("group norm channel kernel launch");
-            });
+            return dispatch_float(p.dtype, [&](auto tag) -> hmc_status { return fold_by_channel(rows.partials, tag); });
+        }
+        if (resident.t.v > 0) {
+            ResidentBackwardArgs b{};
+            b.dsrc = a.dsrc;
+            b.src = a.src;
+            b.dout = a.dout;
+            b.mean = a.mean;
+            b.rstd = a.rstd;
+            b.wdsrc = a.wdsrc;
+            b.wsrc = a.wsrc;
+            b.wdout = a.wdout;
+            b.mean_n = a.mean_n;
+            b.mean_g = a.mean_g;
+            b.rstd_n = a.rstd_n;
+            b.rstd_g = a.rstd_g;
+            b.r = resident;
+            b.samples = p.samples;
+            b.positions = p.positions;
+            b.columns = resident_columns(p, resident);
+            b.affine = affine;
+            b.by_channel = sums_wanted ? workspace : nullptr;
+            s = launch_resident_backward(ctx, p.dtype, activation, b);
+            if (s != HMC_OK || !sums_wanted) return s;
+            return dispatch_float(p.dtype, [&](auto tag) -> hmc_status { return fold_by_channel(b.columns * resident.cluster, tag); });
         }
         a.t = plan.t;
         a.cut = plan.sums;
