@@ -268,7 +268,8 @@ int64_t resident_columns(const Problem &p, const Resident &r) {
     int64_t wanted = ceil_div(kBlocksWanted, r.t.tiles * r.cluster);
     const int64_t least = ceil_div(p.samples, 64);  // samples whose sums one block keeps in the computation type
     if (wanted < least) wanted = least;
-    return wanted < p.samples ? wanted : p.samples;
+    if (wanted >= p.samples) return p.samples;
+    return ceil_div(p.samples, ceil_div(p.samples, wanted));  // the same number of samples for all but the last
 }
 
 }  // namespace

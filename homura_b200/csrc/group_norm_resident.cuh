@@ -19,7 +19,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kResidentCluster = 8;
 constexpr int kResidentShared = 216 * 1024;   // dynamic shared memory of a block at most
-constexpr int kResidentWanted = 100 * 1024;   // two blocks an SM
+constexpr int kResidentWanted = 112 * 1024;   // two blocks an SM
 
 struct Resident {
     Tiling t;           // v = 0: does not fit

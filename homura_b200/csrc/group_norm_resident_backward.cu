@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(kBlock, 2) resident_backward_kernel(const __gr
         C mean[V], rstd[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int64_t group = tile.group + (tx * V + i) / tile.part;
+            const int64_t group = tile.group + column_of.group[i];
             mean[i] = live ? reinterpret_cast<const C *>(a.mean)[sample * a.mean_n + group * a.mean_g] : C(0);
             rstd[i] = live ? reinterpret_cast<const C *>(a.rstd)[sample * a.rstd_n + group * a.rstd_g] : C(0);
         }
