@@ -13,12 +13,15 @@ struct ForwardArgs {
     Walk wout, wgate, wx, winitial, wlast;
     int64_t time, channels, tiles, items;
     int32_t warps_time;
+    int *status;
 };
 
-constexpr int kStages = 3;
+constexpr int kStages = 2;
+// Blocks on an SM: four with eight rows a lane; with sixteen, for launches that fill no more, two.
+template <class T> constexpr int per_sm(int rows) { return sizeof(T) == 8 || rows > 8 ? 2 : 4; }
 
 template <class T, int V, int R, int COPY, bool SIG, bool COMP>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kernel(const __grid_constant__ ForwardArgs a) {
+__global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const __grid_constant__ ForwardArgs a) {
     using C = typename Comp<T>::C;
     using G = Ring<T, V, COPY>;
     __shared__ Exchange<C, V> shared;
@@ -29,8 +32,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kern
     const bool alone = a.warps_time == 1 && p.cluster == 1;
     const int64_t round = static_cast<int64_t>(R) * a.warps_time * p.cluster;
     const int64_t mine = static_cast<int64_t>(R) * (p.rank * a.warps_time + p.wt);
-    if (p.cluster > 1) cg::this_cluster().sync();  // every block runs before anyone writes to its shared memory
-    int generation = 0;
+    begin_exchange(shared, p);
+    uint32_t rounds = 0;
+    bool gave_up = false;
     for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
         const int64_t batch = item / a.tiles;
         const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
@@ -52,25 +56,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kern
         // rows of this warp from t0 on that exist, R at most
         const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
         Pack<T, V> rg[R], rx[R];
+        // the next round's rows (one call a round, in order)
+        const int64_t gate_round = round * a.wgate.t, x_round = round * a.wx.t;
+        const int ahead = COPY > 0 ? G::row() : 0;
+        const T *pg = gate + (mine + ahead) * a.wgate.t, *px = x + (mine + ahead) * a.wx.t;
         const auto fetch = [&](int64_t t0, int stage) {
             const int n = loads ? count(t0) : 0;
             if constexpr (COPY > 0) {
-                copy_rows<T, V, COPY, R>(ring + stage * kStage, 0, gate + (t0 + G::row()) * a.wgate.t, a.wgate.t, n);
-                copy_rows<T, V, COPY, R>(ring + stage * kStage, R, x + (t0 + G::row()) * a.wx.t, a.wx.t, n);
+                copy_rows<T, V, COPY, R>(ring + stage * kStage, 0, pg, a.wgate.t, n);
+                copy_rows<T, V, COPY, R>(ring + stage * kStage, R, px, a.wx.t, n);
                 async_copy_commit();
             } else {
-                const T *pg = gate + t0 * a.wgate.t, *px = x + t0 * a.wx.t;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (r < n) {
-                        rg[r] = load_pack<T, V>(pg);
-                        rx[r] = load_pack<T, V>(px);
+                        rg[r] = load_pack<T, V>(pg + r * a.wgate.t);
+                        rx[r] = load_pack<T, V>(px + r * a.wx.t);
                     }
-                    pg += a.wgate.t;
-                    px += a.wx.t;
                 }
             }
+            pg += gate_round;
+            px += x_round;
         };
+        T *po = out + mine * a.wout.t;
+        const int64_t out_round = round * a.wout.t;
         int stage = 0;
         if constexpr (COPY > 0) {
 #pragma unroll
@@ -128,27 +137,30 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kern
                         s[i].a *= ca[r][i];
                     }
                 }
-                exchange(shared, p, a.warps_time, generation, s, h, carry);
-                generation ^= 1;
+                exchange(shared, p, a.warps_time, rounds, base == 0, s, h, carry, a.status, gave_up);
             }
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;
-                T *po = out + t0 * a.wout.t;
+                T *to = po;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (kWhole || r < n) {
 #pragma unroll
                         for (int i = 0; i < V; ++i) h[i] = m_fma(ca[r][i], h[i], cu[r][i]);
-                        if (live) store_pack<T, V>(po, h);
+                        if (live) store_pack<T, V>(to, h);
                     }
-                    po += a.wout.t;
+                    to += a.wout.t;
                 }
             };
             if (n == R) write(std::true_type{});
             else write(std::false_type{});
+            po += out_round;
             if (alone) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) carry[i] = h[i];
+            } else {
+                leave_carry(shared, p, a.warps_time, rounds, h);
+                ++rounds;
             }
             if (a.last != nullptr && live && n > 0 && t0 + n == a.time) {
 #pragma unroll
@@ -160,11 +172,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 3) forward_kern
             for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = carry[i];
         }
     }
+    end_exchange(p);
 }
 
 template <class T, int V, int R, int COPY>
 hmc_status launch_forward(hmc_context_t ctx, ForwardArgs &a, int64_t batch, int32_t flags) {
-    const Shape shape = plan_launch(batch, a.time, a.channels, V, R);
+    const Shape shape = plan_launch(batch, a.time, a.channels, V, R, per_sm<T>(R));
     a.tiles = shape.tiles;
     a.items = shape.items;
     a.warps_time = shape.warps_time;
@@ -214,6 +227,7 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
         a.wlast = walk_state(last);
         a.time = time;
         a.channels = channels;
+        a.status = ctx->status;
         const bool pairs = layer_vectors(out, 4) && layer_vectors(gate, 4) && layer_vectors(x, 4);
         const bool wide = layer_vectors(gate, 16) && layer_vectors(x, 16) && layer_vectors(out, 4);
         return dispatch_float(dt, [&](auto tag) -> hmc_status {
@@ -223,6 +237,12 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
                 if (!pairs) return time == 1 ? launch_forward<T, 1, 1, 0>(ctx, a, batch, flags) : launch_forward<T, 1, 8, 0>(ctx, a, batch, flags);
             }
             if (time == 1) return launch_forward<T, V, 1, 0>(ctx, a, batch, flags);
+            if constexpr (sizeof(T) < 8) {
+                // Sixteen rows a lane halve the exchanges, where two blocks an SM are all there is to run: with eight warps
+                // along time and no cluster the launch has batch * channel tiles blocks.
+                const bool few = batch * ceil_div(channels, int64_t{32} * V) <= 148 * 2;
+                if (few) return wide ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);
+            }
             return wide ? launch_forward<T, V, 8, 16>(ctx, a, batch, flags) : launch_forward<T, V, 8, kWord>(ctx, a, batch, flags);
         });
     });

@@ -10,8 +10,9 @@
 // and 8 / WT the channels; where batch * channels leave SMs idle, up to eight blocks of a cluster divide the time axis
 // further. A round is then R * WT * cluster rows:
 //   1. every lane folds its rows to (A, B): v after the rows = A * (v before) + B;
-//   2. warps leave (A, B) in shared memory, blocks leave their fold in every block's shared memory of the cluster
-//      (distributed shared memory), one barrier each;
+//   2. warps leave (A, B) in shared memory; the blocks of a cluster send their fold to every block of it (asynchronous
+//      stores into distributed shared memory that count themselves off on the receiver's mbarrier: a cluster barrier
+//      would wait for the results' stores to global memory as well);
 //   3. every lane folds what lies before its rows, always in the order of time, onto the round's carry, and walks its rows
 //      once more from registers, now from the true value, writing the results.
 // No block waits for a block outside its cluster, nothing is read twice, and the order of the folds is fixed by the sizes.
@@ -131,21 +132,19 @@ struct Shape {
     unsigned grid;
 };
 
-// WT and the cluster grow until the launch has about sixteen warps an SM, but not beyond what the time axis can feed. The
-// constant is B200's SM count, not the device's, so that the order of folding is the same everywhere.
-inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, int v, int rows) {
-    constexpr int64_t kEnough = 148 * 16;
+// WT and the cluster grow while every block still finds a place at once, `per_sm` on an SM, and the time axis feeds them:
+// a second, partly filled wave costs more than the warps it brings. The constant is B200's SM count, not the device's, so
+// that the order of folding is the same everywhere.
+inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, int v, int rows, int per_sm) {
+    const int64_t places = int64_t{148} * per_sm;
     Shape s{1, 1, 0, 0, 0};
     const int64_t warps = batch * ceil_div(channels, int64_t{32} * v);  // (both counts are below 2^62 / (32 v))
-    int64_t have = warps;
-    while (have < kEnough && s.warps_time < kWarps && static_cast<int64_t>(s.warps_time) * rows < time) {
+    while (s.warps_time < kWarps && ceil_div(warps, kWarps / (s.warps_time * 2)) <= places && static_cast<int64_t>(s.warps_time) * rows < time) {
         s.warps_time *= 2;
-        have *= 2;
     }
-    while (have < kEnough && s.warps_time == kWarps && s.cluster < kMaxCluster &&
+    while (s.warps_time == kWarps && s.cluster < kMaxCluster && warps * s.cluster * 2 <= places &&
            static_cast<int64_t>(s.warps_time) * s.cluster * rows < time) {
         s.cluster *= 2;
-        have *= 2;
     }
     s.tiles = ceil_div(channels, int64_t{32} * v * (kWarps / s.warps_time));
     s.items = batch * s.tiles;
@@ -246,19 +245,76 @@ template <int V> __device__ __forceinline__ Place place(int warps_time) {
     return p;
 }
 
-// Shared memory of the exchange, two generations so that one barrier a round is enough: a generation is written again
-// two rounds later, after the barrier of the round between, which every reader has reached by then.
-template <class C, int V> struct Exchange {
-    alignas(16) Step<C> warp[2][kWarps][32 * V];
-    alignas(16) Step<C> block[2][kMaxCluster][32 * V];
+// Shared memory of the exchange, two generations: one is written again two rounds later, behind a barrier (or the arrival
+// of the next round's folds) that every reader has passed by then.
+template <class C, int V> struct alignas(16) Exchange {
+    Step<C> warp[2][kWarps][32 * V];
+    Step<C> block[2][kMaxCluster][32 * V];
+    C carry[2][kWarps][32 * V];   // by the warp's place along channels
+    alignas(8) uint64_t arrived[2];
 };
 
-// Step 2 and the folds of step 3: `mine` is what this lane's rows do; v enters as the round's carry and leaves as the
-// value before this lane's rows; carry leaves as the value after the round.
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Before the first round; every thread of the cluster.
+template <class C, int V> __device__ __forceinline__ void begin_exchange(Exchange<C, V> &x, const Place &p) {
+    if (p.cluster == 1) return;
+    if (threadIdx.x == 0) {
+        for (int g = 0; g < 2; ++g) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[g])) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    cg::this_cluster().sync();  // every block runs, its barriers stand, before anyone writes to its shared memory
+}
+// After the last: no block ends while another may still write to it.
+__device__ __forceinline__ void end_exchange(const Place &p) {
+    if (p.cluster > 1) cg::this_cluster().sync();
+}
+
+// One lane's V steps to the same place of another block, counted off on that block's mbarrier.
+template <class C, int V> __device__ __forceinline__ void send(const Step<C> *mine, uint64_t *arrived, int block, const Pack<Step<C>, V> &value) {
+    uint32_t to, at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(shared_address(mine)), "r"(block));
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(shared_address(arrived)), "r"(block));
+    constexpr int kWords = static_cast<int>(sizeof(Step<C>)) * V / 8;
+    uint64_t w[kWords];
+    memcpy(w, &value, sizeof w);
+    if constexpr (kWords == 1) {
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(w[0]), "r"(at) : "memory");
+    } else {
+        static_assert(kWords == 2, "one or two words");
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(to), "l"(w[0]), "l"(w[1]), "r"(at)
+                     : "memory");
+    }
+}
+
+constexpr int kPollLimit = 1 << 22;
+
+// A wait that gives up: no block waits for ever for one that never sends. `status` is the context's word; once a thread has
+// given up it waits no more.
+__device__ __forceinline__ void await(uint64_t *arrived, uint32_t parity, int *status, bool &gave_up) {
+    if (gave_up) return;
+    const uint32_t at = shared_address(arrived);
+    for (int poll = 0; poll < kPollLimit; ++poll) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(at), "r"(parity)
+            : "memory");
+        if (done) return;
+    }
+    gave_up = true;
+    atomicExch(status, 1);
+}
+
+// Step 2 and the folds of step 3: `mine` is what this lane's rows do; v leaves as the value before this lane's rows. Within a
+// block the round's first value is what the last warp along time ended the round before with (left by leave_carry); a
+// cluster folds every block's sum onto the carry that each lane keeps.
 template <class C, int V>
-__device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, int generation, const Step<C> (&mine)[V],
-                                         C (&v)[V], C (&carry)[V]) {
+__device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, bool first_round,
+                                         const Step<C> (&mine)[V], C (&v)[V], C (&carry)[V], int *status, bool &gave_up) {
     using Pair = Pack<Step<C>, V>;
+    const uint32_t generation = round & 1u;
     Step<C>(&warps)[kWarps][32 * V] = x.warp[generation];
     const auto at = [&](const Step<C> (&row)[32 * V]) { return *reinterpret_cast<const Pair *>(&row[p.slot]); };
     const int first = p.wc * warps_time;
@@ -270,13 +326,16 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
     }
     __syncthreads();
     if (p.cluster > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
+        if (threadIdx.x == 0) {
+            asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&x.arrived[generation])),
+                         "r"(static_cast<uint32_t>(p.cluster * 32 * V * sizeof(Step<C>)))
+                         : "memory");
+        }
         // (a cluster is used with all eight warps along time only, so a block has one tile of channels; warp w brings the
         // block's fold to block w)
         if (p.wt < p.cluster) {
-            Step<C>(*there)[32 * V] = cluster.map_shared_rank(x.block[generation], p.wt);
             Pair t = at(warps[0]);
-#pragma unroll 4
+#pragma unroll
             for (int w = 1; w < kWarps; ++w) {
                 const Pair s = at(warps[w]);
 #pragma unroll
@@ -287,35 +346,38 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) t.v[i].a = finite(t.v[i].a);
-            *reinterpret_cast<Pair *>(&there[p.rank][p.slot]) = t;
+            send<C, V>(&x.block[generation][p.rank][p.slot], &x.arrived[generation], p.wt, t);
         }
-        cluster.sync();
+        await(&x.arrived[generation], (round >> 1) & 1u, status, gave_up);
 #pragma unroll 4
         for (int k = 0; k < p.cluster; ++k) {
             const Pair s = at(x.block[generation][k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (k == p.rank) v[i] = carry[i];
                 carry[i] = fold(s.v[i], carry[i]);
-                if (k < p.rank) v[i] = carry[i];
             }
         }
-#pragma unroll 4
-        for (int w = 0; w < p.wt; ++w) {
-            const Pair s = at(warps[w]);
+    } else if (!first_round) {
+        const Pack<C, V> c = *reinterpret_cast<const Pack<C, V> *>(&x.carry[generation][p.wc][p.slot]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = fold(s.v[i], v[i]);
-        }
-    } else {
-#pragma unroll 4
-        for (int w = 0; w < warps_time; ++w) {
-            const Pair s = at(warps[first + w]);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                carry[i] = fold(s.v[i], carry[i]);
-                if (w < p.wt) v[i] = carry[i];
-            }
-        }
+        for (int i = 0; i < V; ++i) v[i] = c.v[i];
     }
+#pragma unroll 4
+    for (int w = 0; w < p.wt; ++w) {
+        const Pair s = at(warps[first + w]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fold(s.v[i], v[i]);
+    }
+}
+// The last warp along time leaves its last value for the next round of the block.
+template <class C, int V>
+__device__ __forceinline__ void leave_carry(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, const C (&v)[V]) {
+    if (p.cluster > 1 || p.wt != warps_time - 1) return;
+    Pack<C, V> c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) c.v[i] = v[i];
+    *reinterpret_cast<Pack<C, V> *>(&x.carry[(round + 1) & 1u][p.wc][p.slot]) = c;
 }
 
 }  // namespace recur

@@ -16,13 +16,15 @@ struct BackwardArgs {
     Walk wdgate, wdx, wdinitial, wgate, wx, wout, wdout, winitial, wdlast;
     int64_t time, channels, tiles, items;
     int32_t warps_time;
+    int *status;
 };
 
 constexpr int kStages = 2;
+template <class T> constexpr int kPerSm = sizeof(T) == 8 ? 1 : 2;  // blocks on an SM
 template <int R, bool COMP> constexpr int kStageRows = (COMP ? 4 : 3) * R + 1;
 
 template <class T, int V, int R, int COPY, bool SIG, bool COMP>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_kernel(const __grid_constant__ BackwardArgs a) {
+__global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __grid_constant__ BackwardArgs a) {
     using C = typename Comp<T>::C;
     using G = Ring<T, V, COPY>;
     __shared__ Exchange<C, V> shared;
@@ -34,8 +36,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_ker
     const bool alone = a.warps_time == 1 && p.cluster == 1;
     const int64_t round = static_cast<int64_t>(R) * a.warps_time * p.cluster;
     const int64_t mine = static_cast<int64_t>(R) * (p.rank * a.warps_time + p.wt);
-    if (p.cluster > 1) cg::this_cluster().sync();  // every block runs before anyone writes to its shared memory
-    int generation = 0;
+    begin_exchange(shared, p);
+    uint32_t rounds = 0;
+    bool gave_up = false;
     for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
         const int64_t batch = item / a.tiles;
         const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
@@ -59,30 +62,40 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_ker
         // rows of this warp from t0 on that exist, R at most
         const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
         Pack<T, V> direct[COPY > 0 ? 1 : kStageRows<R, COMP>];
+        // the next round's rows (one call a round, in order)
+        const int64_t gate_round = round * a.wgate.t, dout_round = round * a.wdout.t, out_round = round * a.wout.t, x_round = round * a.wx.t;
+        const int64_t ahead = mine + (COPY > 0 ? G::row() : 0);
+        const T *pgate = gate + ahead * a.wgate.t, *pdout = dout + ahead * a.wdout.t, *pout = out + (ahead + 1) * a.wout.t;
+        const T *px = COMP ? x + ahead * a.wx.t : nullptr;
         const auto fetch = [&](int64_t t0, int stage) {
             const int n = loads ? count(t0) : 0, states = loads ? count(t0 + 1) : 0, before = n > 0 && t0 > 0 ? 1 : 0;
             if constexpr (COPY > 0) {
                 unsigned char *to = ring + stage * kStage;
-                const int64_t row = t0 + G::row();
-                copy_rows<T, V, COPY, 1>(to, kGate, gate + (row - 1) * a.wgate.t, a.wgate.t, before);
-                copy_rows<T, V, COPY, R>(to, kGate + 1, gate + row * a.wgate.t, a.wgate.t, n);
-                copy_rows<T, V, COPY, R>(to, kDout, dout + row * a.wdout.t, a.wdout.t, n);
-                copy_rows<T, V, COPY, R>(to, kState, out + (row + 1) * a.wout.t, a.wout.t, states);
-                if constexpr (COMP) copy_rows<T, V, COPY, R>(to, kX, x + row * a.wx.t, a.wx.t, n);
+                copy_rows<T, V, COPY, 1>(to, kGate, pgate - a.wgate.t, a.wgate.t, before);
+                copy_rows<T, V, COPY, R>(to, kGate + 1, pgate, a.wgate.t, n);
+                copy_rows<T, V, COPY, R>(to, kDout, pdout, a.wdout.t, n);
+                copy_rows<T, V, COPY, R>(to, kState, pout, a.wout.t, states);
+                if constexpr (COMP) copy_rows<T, V, COPY, R>(to, kX, px, a.wx.t, n);
                 async_copy_commit();
             } else {
-                if (before) direct[kGate] = load_pack<T, V>(gate + (t0 - 1) * a.wgate.t);
+                if (before) direct[kGate] = load_pack<T, V>(pgate - a.wgate.t);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (r < n) {
-                        direct[kGate + 1 + r] = load_pack<T, V>(gate + (t0 + r) * a.wgate.t);
-                        direct[kDout + r] = load_pack<T, V>(dout + (t0 + r) * a.wdout.t);
-                        if (r < states) direct[kState + r] = load_pack<T, V>(out + (t0 + r + 1) * a.wout.t);
-                        if constexpr (COMP) direct[kX + r] = load_pack<T, V>(x + (t0 + r) * a.wx.t);
+                        direct[kGate + 1 + r] = load_pack<T, V>(pgate + r * a.wgate.t);
+                        direct[kDout + r] = load_pack<T, V>(pdout + r * a.wdout.t);
+                        if (r < states) direct[kState + r] = load_pack<T, V>(pout + r * a.wout.t);
+                        if constexpr (COMP) direct[kX + r] = load_pack<T, V>(px + r * a.wx.t);
                     }
                 }
             }
+            pgate += gate_round;
+            pdout += dout_round;
+            pout += out_round;
+            if constexpr (COMP) px += x_round;
         };
+        T *pdgate = dgate + mine * a.wdgate.t, *pdx = dx + mine * a.wdx.t;
+        const int64_t dgate_round = round * a.wdgate.t, dx_round = round * a.wdx.t;
         int filled = 0;
         if constexpr (COPY > 0) {
 #pragma unroll
@@ -142,12 +155,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_ker
 #pragma unroll
             for (int i = 0; i < V; ++i) g[i] = carry[i];
             if (!alone) {
-                exchange(shared, p, a.warps_time, generation, s, g, carry);
-                generation ^= 1;
+                exchange(shared, p, a.warps_time, rounds, base == 0, s, g, carry, a.status, gave_up);
             }
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;  // (and the last row in processing order is not among them)
-                T *pg = dgate + t0 * a.wdgate.t, *px = dx + t0 * a.wdx.t;
+                T *to_gate = pdgate, *to_x = pdx;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (kWhole || r < n) {
@@ -172,19 +184,24 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_ker
                             if constexpr (SIG) da[i] = da[i] * (m[r][i].a * m[r][i].rest);
                         }
                         if (live) {
-                            store_pack<T, V>(pg, da);
-                            store_pack<T, V>(px, du);
+                            store_pack<T, V>(to_gate, da);
+                            store_pack<T, V>(to_x, du);
                         }
                     }
-                    pg += a.wdgate.t;
-                    px += a.wdx.t;
+                    to_gate += a.wdgate.t;
+                    to_x += a.wdx.t;
                 }
             };
             if (n == R && !last) write(std::true_type{});
             else write(std::false_type{});
+            pdgate += dgate_round;
+            pdx += dx_round;
             if (alone) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) carry[i] = g[i];
+            } else {
+                leave_carry(shared, p, a.warps_time, rounds, g);
+                ++rounds;
             }
         }
         if (a.time == 0 && live && p.rank == 0 && p.wt == 0 && a.dinitial != nullptr) {
@@ -192,11 +209,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 1 : 2) backward_ker
             for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = carry[i];
         }
     }
+    end_exchange(p);
 }
 
 template <class T, int V, int R, int COPY>
 hmc_status launch_backward(hmc_context_t ctx, BackwardArgs &a, int64_t batch, int32_t flags) {
-    const Shape shape = plan_launch(batch, a.time, a.channels, V, R);
+    const Shape shape = plan_launch(batch, a.time, a.channels, V, R, kPerSm<T>);
     a.tiles = shape.tiles;
     a.items = shape.items;
     a.warps_time = shape.warps_time;
@@ -262,6 +280,7 @@ HMC_API hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_t
         a.wdlast = walk_state(dlast);
         a.time = time;
         a.channels = channels;
+        a.status = ctx->status;
         const bool pairs = layer_vectors(dgate, 4) && layer_vectors(dx, 4) && layer_vectors(gate, 4) && layer_vectors(out, 4) &&
                            layer_vectors(dout, 4) && (!complement || layer_vectors(x, 4));
         const bool wide = layer_vectors(gate, 16) && layer_vectors(out, 16) && layer_vectors(dout, 16) &&
