@@ -46,12 +46,12 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
         const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + column * a.wgate.c;
         const T *x = reinterpret_cast<const T *>(a.x) + batch * a.wx.b + column * a.wx.c;
         T *out = reinterpret_cast<T *>(a.out) + batch * a.wout.b + channel * a.wout.c;
-        C carry[V];
+        Vec<C, V> carry;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            carry[i] = C(0);
+            carry.v[i] = C(0);
             if (a.initial != nullptr && live)
-                carry[i] = reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
+                carry.v[i] = reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
         }
         // rows of this warp from t0 on that exist, R at most
         const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
@@ -107,37 +107,32 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
             // All R rows exist for most warps (`whole`, the same for a warp's lanes): that form has no conditions in it. The
             // barriers of the exchange stand outside. Lanes beyond the last channel compute on whatever their registers
             // hold and write nothing.
-            C ca[R][V], cu[R][V];
-            Step<C> s[V];
+            Vec<C, V> ca[R], cu[R];
             const auto read = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const Gate<C> g = gate_of<SIG>(rg[r].v[i]);
-                        ca[r][i] = kWhole || r < n ? g.a : C(1);
-                        cu[r][i] = kWhole || r < n ? (COMP ? g.rest * up(rx[r].v[i]) : up(rx[r].v[i])) : C(0);
+                    if (kWhole || r < n) {
+                        const Gates<C, V> g = gates_of<SIG, T, V>(rg[r]);
+                        ca[r] = g.a;
+                        cu[r] = COMP ? vmul(g.rest, widen<T, V>(rx[r])) : widen<T, V>(rx[r]);
+                    } else {
+                        ca[r] = splat<C, V>(C(1));
+                        cu[r] = splat<C, V>(C(0));
                     }
                 }
             };
             if (n == R) read(std::true_type{});
             else read(std::false_type{});
-            C h[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) h[i] = carry[i];
+            Vec<C, V> h = carry;
             if (!alone) {
+                Vec<C, V> product = ca[0], sum = vfma(ca[0], splat<C, V>(C(0)), cu[0]);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s[i].a = ca[0][i];
-                    s[i].b = m_fma(ca[0][i], C(0), cu[0][i]);
-#pragma unroll
-                    for (int r = 1; r < R; ++r) {
-                        s[i].b = m_fma(ca[r][i], s[i].b, cu[r][i]);
-                        s[i].a *= ca[r][i];
-                    }
+                for (int r = 1; r < R; ++r) {
+                    sum = vfma(ca[r], sum, cu[r]);
+                    product = vmul(product, ca[r]);
                 }
-                exchange(shared, p, a.warps_time, rounds, base == 0, s, h, carry, a.status, gave_up);
+                exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, h, carry, a.status, gave_up);
             }
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;
@@ -145,8 +140,7 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (kWhole || r < n) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) h[i] = m_fma(ca[r][i], h[i], cu[r][i]);
+                        h = vfma(ca[r], h, cu[r]);
                         if (live) store_pack<T, V>(to, h);
                     }
                     to += a.wout.t;
@@ -156,20 +150,19 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
             else write(std::false_type{});
             po += out_round;
             if (alone) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) carry[i] = h[i];
+                carry = h;
             } else {
                 leave_carry(shared, p, a.warps_time, rounds, h);
                 ++rounds;
             }
             if (a.last != nullptr && live && n > 0 && t0 + n == a.time) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = h[i];
+                for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = h.v[i];
             }
         }
         if (a.time == 0 && live && p.rank == 0 && p.wt == 0 && a.last != nullptr) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = carry[i];
+            for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = carry.v[i];
         }
     }
     end_exchange(p);
@@ -238,9 +231,8 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
             }
             if (time == 1) return launch_forward<T, V, 1, 0>(ctx, a, batch, flags);
             if constexpr (sizeof(T) < 8) {
-                // Sixteen rows a lane halve the exchanges, where two blocks an SM are all there is to run: with eight warps
-                // along time and no cluster the launch has batch * channel tiles blocks.
-                const bool few = batch * ceil_div(channels, int64_t{32} * V) <= 148 * 2;
+                // Sixteen rows a lane halve the exchanges, two blocks an SM then: where that many blocks take all channels.
+                const bool few = batch * ceil_div(channels, int64_t{32} * V) <= int64_t{148} * 2 * kWarps;
                 if (few) return wide ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);
             }
             return wide ? launch_forward<T, V, 8, 16>(ctx, a, batch, flags) : launch_forward<T, V, 8, kWord>(ctx, a, batch, flags);

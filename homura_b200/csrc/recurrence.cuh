@@ -49,41 +49,122 @@ struct Walk {
     int64_t b, t, c;
 };
 
-// a and 1 - a of a gate, each with full relative precision however close to 0 or 1 a is.
-template <class C> struct Gate {
-    C a, rest;
+// V values of the computation type. Pairs of f32 go through the packed instructions, two products or sums an issue.
+template <class C, int V> struct Vec {
+    C v[V];
 };
-template <bool SIG, class T> __device__ __forceinline__ Gate<typename Comp<T>::C> gate_of(T stored) {
-    using C = typename Comp<T>::C;
-    const C g = up(stored);
-    if constexpr (!SIG) {
-        return Gate<C>{g, C(1) - g};
-    } else if constexpr (sizeof(T) == 2) {
-        // rounded to at most 11 bits later. e = exp(-g), held below 2^126 so that both approximations stay in range (a is
-        // 2^-126 then, where it should be less); the minimum passes a NaN on
-        float t = g * -1.44269504088896341f, e, a;
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"(t), "f"(126.0f));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.0f + e));
-        return Gate<C>{a, e * a};
+template <class C, int V> __device__ __forceinline__ Vec<C, V> vfma(const Vec<C, V> &a, const Vec<C, V> &b, const Vec<C, V> &c) {
+    Vec<C, V> r;
+    if constexpr (std::is_same_v<C, float> && V == 2) {
+        asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+            "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+            : "=f"(r.v[0]), "=f"(r.v[1])
+            : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]), "f"(c.v[0]), "f"(c.v[1]));
     } else {
-        const C e = exp(-m_abs(g)), large = C(1) / (C(1) + e), small = e * large;
-        return g > C(0) ? Gate<C>{large, small} : Gate<C>{small, large};
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = m_fma(a.v[i], b.v[i], c.v[i]);
     }
+    return r;
+}
+template <class C, int V> __device__ __forceinline__ Vec<C, V> vmul(const Vec<C, V> &a, const Vec<C, V> &b) {
+    Vec<C, V> r;
+    if constexpr (std::is_same_v<C, float> && V == 2) {
+        asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+            : "=f"(r.v[0]), "=f"(r.v[1])
+            : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = a.v[i] * b.v[i];
+    }
+    return r;
+}
+template <class C, int V> __device__ __forceinline__ Vec<C, V> vadd(const Vec<C, V> &a, const Vec<C, V> &b) {
+    Vec<C, V> r;
+    if constexpr (std::is_same_v<C, float> && V == 2) {
+        asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+            : "=f"(r.v[0]), "=f"(r.v[1])
+            : "f"(a.v[0]), "f"(a.v[1]), "f"(b.v[0]), "f"(b.v[1]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = a.v[i] + b.v[i];
+    }
+    return r;
+}
+template <class C, int V> __device__ __forceinline__ Vec<C, V> splat(C c) {
+    Vec<C, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = c;
+    return r;
+}
+template <class T, int V> __device__ __forceinline__ Vec<typename Comp<T>::C, V> widen(const Pack<T, V> &p) {
+    Vec<typename Comp<T>::C, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = up(p.v[i]);
+    return r;
+}
+
+// a and 1 - a of V gates, each with full relative precision however close to 0 or 1 a is.
+template <class C, int V> struct Gates {
+    Vec<C, V> a, rest;
+};
+// Logits of half types held at -87 or above, NaN passed on.
+__device__ __forceinline__ uint32_t at_least_87(uint32_t pair, F16) {
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(pair) : "r"(0xD570D570u));
+    return pair;
+}
+__device__ __forceinline__ uint32_t at_least_87(uint32_t pair, BF16) {
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(pair) : "r"(0xC2AEC2AEu));
+    return pair;
+}
+template <bool SIG, class T, int V> __device__ __forceinline__ Gates<typename Comp<T>::C, V> gates_of(Pack<T, V> stored) {
+    using C = typename Comp<T>::C;
+    Gates<C, V> r;
+    if constexpr (!SIG) {
+        r.a = widen<T, V>(stored);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.rest.v[i] = C(1) - r.a.v[i];
+    } else if constexpr (sizeof(T) == 2) {
+        // rounded to at most 11 bits later. e = exp(-g) stays below 2^126, so that both approximations stay in range (a is
+        // e^-87 where it should be less)
+        if constexpr (V == 2) {
+            uint32_t pair;
+            memcpy(&pair, &stored, 4);
+            pair = at_least_87(pair, T{});
+            memcpy(&stored, &pair, 4);
+        }
+        Vec<C, V> t = widen<T, V>(stored), e;
+        if constexpr (V == 1) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.v[0]) : "f"(-87.0f));
+        t = vmul(t, splat<C, V>(-1.44269504088896341f));
+#pragma unroll
+        for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v[i]) : "f"(t.v[i]));
+        t = vadd(e, splat<C, V>(1.0f));
+#pragma unroll
+        for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.a.v[i]) : "f"(t.v[i]));
+        r.rest = vmul(e, r.a);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const C g = up(stored.v[i]);
+            const C e = exp(-m_abs(g)), large = C(1) / (C(1) + e), small = e * large;
+            r.a.v[i] = g > C(0) ? large : small;
+            r.rest.v[i] = g > C(0) ? small : large;
+        }
+    }
+    return r;
 }
 
 // V elements at p, the channels `c` elements apart (V > 1 only where c is 1 and the access aligned).
 template <class T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
     return *reinterpret_cast<const Pack<T, V> *>(p);
 }
-template <class T, int V> __device__ __forceinline__ void store_pack(T *p, const typename Comp<T>::C (&v)[V]) {
+template <class T, int V> __device__ __forceinline__ void store_pack(T *p, const Vec<typename Comp<T>::C, V> &v) {
     Pack<T, V> r;
     if constexpr (V % 2 == 0 && sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < V; i += 2) down2(r.v[i], r.v[i + 1], v[i], v[i + 1]);
+        for (int i = 0; i < V; i += 2) down2(r.v[i], r.v[i + 1], v.v[i], v.v[i + 1]);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) r.v[i] = down<T>(v[i]);
+        for (int i = 0; i < V; ++i) r.v[i] = down<T>(v.v[i]);
     }
     *reinterpret_cast<Pack<T, V> *>(p) = r;
 }
@@ -307,12 +388,13 @@ __device__ __forceinline__ void await(uint64_t *arrived, uint32_t parity, int *s
     atomicExch(status, 1);
 }
 
-// Step 2 and the folds of step 3: `mine` is what this lane's rows do; v leaves as the value before this lane's rows. Within a
+// Step 2 and the folds of step 3: (a, b) is what this lane's rows do; v enters as the
+// item's first value and leaves as the value before this lane's rows. Within a
 // block the round's first value is what the last warp along time ended the round before with (left by leave_carry); a
 // cluster folds every block's sum onto the carry that each lane keeps.
 template <class C, int V>
 __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, bool first_round,
-                                         const Step<C> (&mine)[V], C (&v)[V], C (&carry)[V], int *status, bool &gave_up) {
+                                         const Vec<C, V> &a, const Vec<C, V> &b, Vec<C, V> &v, Vec<C, V> &carry, int *status, bool &gave_up) {
     using Pair = Pack<Step<C>, V>;
     const uint32_t generation = round & 1u;
     Step<C>(&warps)[kWarps][32 * V] = x.warp[generation];
@@ -321,7 +403,7 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
     {
         Pair mine_packed;
 #pragma unroll
-        for (int i = 0; i < V; ++i) mine_packed.v[i] = Step<C>{finite(mine[i].a), mine[i].b};
+        for (int i = 0; i < V; ++i) mine_packed.v[i] = Step<C>{finite(a.v[i]), b.v[i]};
         *reinterpret_cast<Pair *>(&warps[first + p.wt][p.slot]) = mine_packed;
     }
     __syncthreads();
@@ -354,29 +436,29 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
             const Pair s = at(x.block[generation][k]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                if (k == p.rank) v[i] = carry[i];
-                carry[i] = fold(s.v[i], carry[i]);
+                if (k == p.rank) v.v[i] = carry.v[i];
+                carry.v[i] = fold(s.v[i], carry.v[i]);
             }
         }
     } else if (!first_round) {
         const Pack<C, V> c = *reinterpret_cast<const Pack<C, V> *>(&x.carry[generation][p.wc][p.slot]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = c.v[i];
+        for (int i = 0; i < V; ++i) v.v[i] = c.v[i];
     }
 #pragma unroll 4
     for (int w = 0; w < p.wt; ++w) {
         const Pair s = at(warps[first + w]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = fold(s.v[i], v[i]);
+        for (int i = 0; i < V; ++i) v.v[i] = fold(s.v[i], v.v[i]);
     }
 }
 // The last warp along time leaves its last value for the next round of the block.
 template <class C, int V>
-__device__ __forceinline__ void leave_carry(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, const C (&v)[V]) {
+__device__ __forceinline__ void leave_carry(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, const Vec<C, V> &v) {
     if (p.cluster > 1 || p.wt != warps_time - 1) return;
     Pack<C, V> c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) c.v[i] = v[i];
+    for (int i = 0; i < V; ++i) c.v[i] = v.v[i];
     *reinterpret_cast<Pack<C, V> *>(&x.carry[(round + 1) & 1u][p.wc][p.slot]) = c;
 }
 

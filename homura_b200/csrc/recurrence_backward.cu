@@ -53,11 +53,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
         const T *dout = reinterpret_cast<const T *>(a.dout) + batch * a.wdout.b + column * a.wdout.c;
         T *dgate = reinterpret_cast<T *>(a.dgate) + batch * a.wdgate.b + channel * a.wdgate.c;
         T *dx = reinterpret_cast<T *>(a.dx) + batch * a.wdx.b + channel * a.wdx.c;
-        C carry[V];
+        Vec<C, V> carry;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            carry[i] = C(0);
-            if (a.dlast != nullptr && live) carry[i] = reinterpret_cast<const C *>(a.dlast)[batch * a.wdlast.b + (channel + i) * a.wdlast.c];
+            carry.v[i] = C(0);
+            if (a.dlast != nullptr && live) carry.v[i] = reinterpret_cast<const C *>(a.dlast)[batch * a.wdlast.b + (channel + i) * a.wdlast.c];
         }
         // rows of this warp from t0 on that exist, R at most
         const auto count = [&](int64_t t0) { return static_cast<int>(a.time - t0 < R ? (a.time - t0 > 0 ? a.time - t0 : 0) : R); };
@@ -124,68 +124,54 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
             // All R rows exist for most warps (`whole`, the same for a warp's lanes): that form has no conditions in it. The
             // barriers of the exchange stand outside. Lanes beyond the last channel compute on whatever there is and write
             // nothing.
-            C first[V];  // the gate of the row before this warp's
-            Gate<C> m[R][V];
-            Step<C> s[V];
+            Vec<C, V> first;  // the gate of the row before this warp's
+            Gates<C, V> m[R];
+            Vec<C, V> product, sum;
             const auto read = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;
-                const Pack<T, V> before = at(kGate);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    first[i] = n > 0 && t0 > 0 ? gate_of<SIG>(before.v[i]).a : C(1);
-                    s[i] = Step<C>{first[i], C(0)};
-                }
+                first = n > 0 && t0 > 0 ? gates_of<SIG, T, V>(at(kGate)).a : splat<C, V>(C(1));
+                product = first;
+                sum = splat<C, V>(C(0));
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const Pack<T, V> g = at(kGate + 1 + r), d = at(kDout + r);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        if (kWhole || r < n) {
-                            m[r][i] = gate_of<SIG>(g.v[i]);
-                            const C c = r == 0 ? first[i] : m[r == 0 ? 0 : r - 1][i].a;
-                            s[i].b = m_fma(c, s[i].b, up(d.v[i]));
-                            if (r > 0) s[i].a *= c;
-                        }
+                    if (kWhole || r < n) {
+                        m[r] = gates_of<SIG, T, V>(at(kGate + 1 + r));
+                        const Vec<C, V> c = r == 0 ? first : m[r == 0 ? 0 : r - 1].a;
+                        sum = vfma(c, sum, widen<T, V>(at(kDout + r)));
+                        if (r > 0) product = vmul(product, c);
                     }
                 }
             };
             if (n == R) read(std::true_type{});
             else read(std::false_type{});
-            C g[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) g[i] = carry[i];
-            if (!alone) {
-                exchange(shared, p, a.warps_time, rounds, base == 0, s, g, carry, a.status, gave_up);
-            }
+            Vec<C, V> g = carry;
+            if (!alone) exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, g, carry, a.status, gave_up);
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;  // (and the last row in processing order is not among them)
                 T *to_gate = pdgate, *to_x = pdx;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (kWhole || r < n) {
-                        const Pack<T, V> d = at(kDout + r), state = at(kState + r), xr = at(COMP ? kX + r : kGate);
-                        C da[V], du[V];
+                        g = vfma(r == 0 ? first : m[r == 0 ? 0 : r - 1].a, g, widen<T, V>(at(kDout + r)));
+                        Vec<C, V> h = widen<T, V>(at(kState + r));
+                        if constexpr (!kWhole) {
+                            if (r + 1 == n && last) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            g[i] = m_fma(r == 0 ? first[i] : m[r == 0 ? 0 : r - 1][i].a, g[i], up(d.v[i]));
-                            C h = up(state.v[i]);
-                            if constexpr (!kWhole) {
-                                if (r + 1 == n && last) {
-                                    h = a.initial == nullptr || !live ? C(0)
-                                                                      : reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
+                                for (int i = 0; i < V; ++i) {
+                                    h.v[i] = a.initial == nullptr || !live ? C(0)
+                                                                           : reinterpret_cast<const C *>(a.initial)[batch * a.winitial.b + (channel + i) * a.winitial.c];
                                     if (a.dinitial != nullptr && live) {
-                                        reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = m[r][i].a * g[i];
+                                        reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = m[r].a.v[i] * g.v[i];
                                     }
                                 }
                             }
-                            if constexpr (COMP) h = h - up(xr.v[i]);
-                            du[i] = COMP ? g[i] * m[r][i].rest : g[i];
-                            da[i] = g[i] * h;
-                            if constexpr (SIG) da[i] = da[i] * (m[r][i].a * m[r][i].rest);
                         }
+                        if constexpr (COMP) h = vfma(widen<T, V>(at(kX + r)), splat<C, V>(C(-1)), h);  // (exact product: h - x)
+                        Vec<C, V> da = vmul(g, h);
+                        if constexpr (SIG) da = vmul(da, vmul(m[r].a, m[r].rest));
                         if (live) {
                             store_pack<T, V>(to_gate, da);
-                            store_pack<T, V>(to_x, du);
+                            store_pack<T, V>(to_x, COMP ? vmul(g, m[r].rest) : g);
                         }
                     }
                     to_gate += a.wdgate.t;
@@ -197,8 +183,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
             pdgate += dgate_round;
             pdx += dx_round;
             if (alone) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) carry[i] = g[i];
+                carry = g;
             } else {
                 leave_carry(shared, p, a.warps_time, rounds, g);
                 ++rounds;
@@ -206,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
         }
         if (a.time == 0 && live && p.rank == 0 && p.wt == 0 && a.dinitial != nullptr) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = carry[i];
+            for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = carry.v[i];
         }
     }
     end_exchange(p);
