@@ -1,9 +1,9 @@
 // Dropout from the counter-based generator (include/homura_cuda_layers.h): the mask of element i is a word of a Philox
 // block named by i alone, so it is recomputed where the gradient needs it and never stored.
 //
-// A thread takes two Philox blocks, eight neighbouring elements, with one vector access per operand. Ten rounds of two
-// wide multiplications per four elements are about 15 integer operations an element beside 4 (bf16, no residual) to 12
-// bytes of traffic.
+// A thread takes two Philox blocks, eight neighbouring elements, at a time. Ten rounds of two wide multiplications and two
+// three-way exclusive ors per four elements are ten integer operations an element beside 4 (bf16, no residual) to 12 bytes
+// of traffic: arithmetic and memory bind alike.
 #include <cmath>
 
 #include "layers.cuh"
@@ -14,19 +14,20 @@ namespace hmc {
 namespace {
 
 constexpr int kDropThreads = 256;
-constexpr int kPer = 8;  // elements a thread takes: two Philox blocks
-
+constexpr int kDropDevices = 64;
+constexpr int kPer = 8;     // neighbouring elements a thread takes at a time: two Philox blocks
 template <class C> struct DropRule {
-    uint64_t seed, offset;
-    uint32_t threshold;  // a word below it drops its element
-    bool all;            // every element is dropped (p rounds to 1)
+    PhiloxKeys keys;
+    uint64_t offset;
+    uint32_t above;  // a word above it keeps its element
     C scale;
 };
 
-template <class T, bool RES>
+// RNG: false where nothing is dropped.
+template <class T, bool RES, bool RNG>
 __device__ __forceinline__ typename Comp<T>::C drop(uint32_t word, T x, T residual, const DropRule<typename Comp<T>::C> &rule) {
     using C = typename Comp<T>::C;
-    const bool keep = word >= rule.threshold && !rule.all;
+    const bool keep = !RNG || word > rule.above;
     // (selected, not multiplied by 0: a dropped NaN or infinity leaves nothing)
     if constexpr (RES) {
         const C r = up(residual);
@@ -36,49 +37,106 @@ __device__ __forceinline__ typename Comp<T>::C drop(uint32_t word, T x, T residu
     }
 }
 
-template <class T, bool RES>
-__global__ void __launch_bounds__(kDropThreads) dropout_flat_kernel(T *out, const T *src, const T *residual, int64_t n, bool vectors,
-                                                                    const DropRule<typename Comp<T>::C> rule) {
+// Eight neighbours from their two Philox blocks, the first of which is 2 * piece.
+template <class T, bool RES, bool RNG>
+__device__ __forceinline__ Pack<T, kPer> drop_piece(int64_t piece, const Pack<T, kPer> &x, const Pack<T, kPer> &r,
+                                                    const DropRule<typename Comp<T>::C> &rule) {
     using C = typename Comp<T>::C;
+    C v[kPer];
+#pragma unroll
+    for (int b = 0; b < kPer / 4; ++b) {
+        Words4 w{};
+        if constexpr (RNG) w = philox_block(rule.offset + static_cast<uint64_t>(piece) * (kPer / 4) + b, rule.keys);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * b + j] = drop<T, RES, RNG>(w.w[j], x.v[4 * b + j], r.v[4 * b + j], rule);
+    }
+    Pack<T, kPer> y;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < kPer; j += 2) down2(y.v[j], y.v[j + 1], v[j], v[j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) y.v[j] = down<T>(v[j]);
+    }
+    return y;
+}
+
+// What is left of a piece element by element: the last one, or all where an operand does not start on 16 bytes.
+template <class T, bool RES, bool RNG>
+__device__ __forceinline__ void drop_ragged(T *out, const T *src, const T *residual, int64_t n, int64_t piece, const DropRule<typename Comp<T>::C> &rule) {
+    Pack<T, kPer> x, r;
+    const int64_t i0 = piece * kPer;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (i0 + j < n) {
+            x.v[j] = src[i0 + j];
+            if constexpr (RES) r.v[j] = residual[i0 + j];
+        }
+    }
+    const Pack<T, kPer> y = drop_piece<T, RES, RNG>(piece, x, r, rule);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (i0 + j < n) out[i0 + j] = y.v[j];
+}
+template <class T, bool RES, bool RNG>
+__global__ void __launch_bounds__(kDropThreads) dropout_ragged_kernel(T *out, const T *src, const T *residual, int64_t n,
+                                                                      const __grid_constant__ DropRule<typename Comp<T>::C> rule) {
     const int64_t pieces = (n + kPer - 1) / kPer;
     for (int64_t piece = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; piece < pieces;
          piece += static_cast<int64_t>(gridDim.x) * kDropThreads) {
-        const int64_t i0 = piece * kPer;
-        const bool whole = vectors && i0 + kPer <= n;
-        Pack<T, kPer> x, r, y;
-        if (whole) {
-            vector_load<T, kPer>(x, src + i0, false);
-            if constexpr (RES) vector_load<T, kPer>(r, residual + i0, false);
-        } else {
+        drop_ragged<T, RES, RNG>(out, src, residual, n, piece, rule);
+    }
+}
+
+// Contiguous operands on 16-byte boundaries: a resident grid walks the pieces, and a thread's next pieces come through a
+// ring in shared memory that its own asynchronous copies fill while it works out the present one's words: the rounds of the
+// generator and the memory's latency overlap without a register spent on data in flight.
+template <class T, bool RES> struct DropRing {
+    static constexpr int kWords = kPer * static_cast<int>(sizeof(T)) / 16;          // copies an operand and piece
+    static constexpr int kPiece = (RES ? 2 : 1) * kWords * kDropThreads * 16;       // bytes a block and piece
+    static constexpr int kStages = kPiece <= 8192 ? 4 : (kPiece <= 16384 ? 3 : 2);  // the one being worked on among them
+    static constexpr int kBytes = kStages * kPiece;                                 // (64 KB at most: F64 with a residual)
+};
+
+template <class T, bool RES, bool RNG>
+__global__ void __launch_bounds__(kDropThreads, sizeof(T) == 8 ? 2 : 4) dropout_flat_kernel(T *out, const T *src, const T *residual, int64_t n,
+                                                                                          const __grid_constant__ DropRule<typename Comp<T>::C> rule) {
+    using G = DropRing<T, RES>;
+    extern __shared__ __align__(16) unsigned char ring[];
+    const int64_t pieces = (n + kPer - 1) / kPer, whole = n / kPer, stride = static_cast<int64_t>(gridDim.x) * kDropThreads;
+    unsigned char *mine = ring + threadIdx.x * 16;  // this thread's copies, kDropThreads * 16 bytes apart
+    const auto fetch = [&](int64_t piece, int stage) {
+        if (piece < whole) {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                if (i0 + j < n) {
-                    x.v[j] = src[i0 + j];
-                    if constexpr (RES) r.v[j] = residual[i0 + j];
+            for (int w = 0; w < G::kWords; ++w) {
+                async_copy_16(mine + stage * G::kPiece + w * (kDropThreads * 16), reinterpret_cast<const char *>(src + piece * kPer) + 16 * w);
+                if constexpr (RES) {
+                    async_copy_16(mine + stage * G::kPiece + (G::kWords + w) * (kDropThreads * 16),
+                                  reinterpret_cast<const char *>(residual + piece * kPer) + 16 * w);
                 }
             }
         }
-        C v[kPer];
+        async_copy_commit();
+    };
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x;
 #pragma unroll
-        for (int b = 0; b < kPer / 4; ++b) {
-            const Words4 w = philox_block(rule.offset + static_cast<uint64_t>(piece) * (kPer / 4) + b, rule.seed);
+    for (int k = 0; k + 1 < G::kStages; ++k) fetch(first + k * stride, k);
+    int stage = 0;
+    for (int64_t piece = first; piece < pieces; piece += stride) {
+        fetch(piece + (G::kStages - 1) * stride, stage == 0 ? G::kStages - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(G::kStages - 1) : "memory");
+        if (piece < whole) {
+            Pack<T, kPer> x, r;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * b + j] = drop<T, RES>(w.w[j], x.v[4 * b + j], r.v[4 * b + j], rule);
-        }
-        if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int j = 0; j < kPer; j += 2) down2(y.v[j], y.v[j + 1], v[j], v[j + 1]);
+            for (int w = 0; w < G::kWords; ++w) {
+                memcpy(reinterpret_cast<char *>(&x) + 16 * w, mine + stage * G::kPiece + w * (kDropThreads * 16), 16);
+                if constexpr (RES) memcpy(reinterpret_cast<char *>(&r) + 16 * w, mine + stage * G::kPiece + (G::kWords + w) * (kDropThreads * 16), 16);
+            }
+            vector_store<T, kPer>(out + piece * kPer, drop_piece<T, RES, RNG>(piece, x, r, rule), false);
         } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) y.v[j] = down<T>(v[j]);
+            drop_ragged<T, RES, RNG>(out, src, residual, n, piece, rule);
         }
-        if (whole) {
-            vector_store<T, kPer>(out + i0, y, false);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (i0 + j < n) out[i0 + j] = y.v[j];
-        }
+        stage = stage + 1 == G::kStages ? 0 : stage + 1;
     }
 }
 
@@ -91,16 +149,16 @@ struct StridedArgs {
     int64_t strides[3][HMC_MAX_DIMS];
 };
 
-template <class T, bool RES>
+template <class T, bool RES, bool RNG>
 __global__ void __launch_bounds__(kDropThreads) dropout_strided_kernel(const __grid_constant__ StridedArgs a,
-                                                                       const DropRule<typename Comp<T>::C> rule) {
+                                                                       const __grid_constant__ DropRule<typename Comp<T>::C> rule) {
     T *out = reinterpret_cast<T *>(a.base[0]);
     const T *src = reinterpret_cast<const T *>(a.base[1]);
     const T *residual = reinterpret_cast<const T *>(a.base[2]);
     const int64_t blocks = (a.n + 3) / 4;
     for (int64_t b = static_cast<int64_t>(blockIdx.x) * kDropThreads + threadIdx.x; b < blocks;
          b += static_cast<int64_t>(gridDim.x) * kDropThreads) {
-        const Words4 w = philox_block(rule.offset + static_cast<uint64_t>(b), rule.seed);
+        const Words4 w = philox_block(rule.offset + static_cast<uint64_t>(b), rule.keys);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             int64_t rest = 4 * b + j;
@@ -114,7 +172,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_strided_kernel(const __g
                 if constexpr (RES) ro += i * a.strides[2][d];
                 rest = q;
             }
-            out[oo] = down<T>(drop<T, RES>(w.w[j], src[so], RES ? residual[ro] : T{}, rule));
+            out[oo] = down<T>(drop<T, RES, RNG>(w.w[j], src[so], RES ? residual[ro] : T{}, rule));
         }
     }
 }
@@ -139,8 +197,8 @@ HMC_API hmc_status hmc_dropout(hmc_context_t ctx, const hmc_tensor_desc *out, co
         if (s != HMC_OK) return s;
         HMC_ENTER(ctx);
         if (n == 0) return HMC_OK;
-        const double threshold = std::nearbyint(p * 4294967296.0);
-        const bool all = threshold >= 4294967296.0;
+        const double threshold = std::nearbyint(p * 4294967296.0);  // words below it drop their element
+        const bool none = threshold < 1.0, all = threshold >= 4294967296.0;
         const int dims = src->ndim;
         auto flat = [&](const hmc_tensor_desc *d) {
             return d == nullptr || dims == 0 || (dims == 1 && (d->strides[0] == 1 || d->sizes[0] == 1));
@@ -154,28 +212,47 @@ HMC_API hmc_status hmc_dropout(hmc_context_t ctx, const hmc_tensor_desc *out, co
         return dispatch_float(src->dtype, [&](auto tag) -> hmc_status {
             using T = decltype(tag);
             using C = typename Comp<T>::C;
-            const DropRule<C> rule{seed, offset, all ? 0u : static_cast<uint32_t>(threshold), all, all ? C(0) : static_cast<C>(1.0 / (1.0 - p))};
-            if (is_flat) {
-                T *o = reinterpret_cast<T *>(layer_base(out));
-                const T *x = reinterpret_cast<const T *>(layer_base(src)), *r = reinterpret_cast<const T *>(layer_base(residual));
-                if (r != nullptr) dropout_flat_kernel<T, true><<<grid, kDropThreads, 0, ctx->stream>>>(o, x, r, n, vectors, rule);
-                else dropout_flat_kernel<T, false><<<grid, kDropThreads, 0, ctx->stream>>>(o, x, r, n, vectors, rule);
-            } else {
-                StridedArgs a{};
-                const hmc_tensor_desc *d[3] = {out, src, residual};
-                a.ndim = dims;
-                a.n = n;
-                for (int k = 0; k < 3; ++k) {
-                    a.base[k] = layer_base(d[k]);
-                    for (int j = 0; j < dims; ++j) {
-                        a.sizes[j] = src->sizes[j];
-                        a.strides[k][j] = d[k] != nullptr ? d[k]->strides[j] : 0;
+            const DropRule<C> rule{philox_keys(seed), offset, none ? 0u : (all ? 0xFFFFFFFFu : static_cast<uint32_t>(threshold) - 1u),
+                                   all ? C(0) : static_cast<C>(1.0 / (1.0 - p))};
+            const auto launch = [&](auto with_residual, auto with_words) -> hmc_status {
+                constexpr bool RES = decltype(with_residual)::value, RNG = decltype(with_words)::value;
+                if (is_flat) {
+                    T *o = reinterpret_cast<T *>(layer_base(out));
+                    const T *x = reinterpret_cast<const T *>(layer_base(src)), *r = reinterpret_cast<const T *>(layer_base(residual));
+                    if (vectors) {
+                        using G = DropRing<T, RES>;
+                        static bool raised[kDropDevices] = {};  // (a race between threads only repeats the call)
+                        if (G::kBytes > 32768 && (ctx->device >= kDropDevices || !raised[ctx->device])) {
+                            HMC_CUDA(cudaFuncSetAttribute(dropout_flat_kernel<T, RES, RNG>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes),
+                                     "shared memory size of the dropout kernel");
+                            if (ctx->device < kDropDevices) raised[ctx->device] = true;
+                        }
+                        const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (sizeof(T) == 8 ? 2 : 4);
+                        const unsigned flat_grid = static_cast<unsigned>(blocks < resident ? blocks : resident);
+                        dropout_flat_kernel<T, RES, RNG><<<flat_grid, kDropThreads, G::kBytes, ctx->stream>>>(o, x, r, n, rule);
+                    } else {
+                        dropout_ragged_kernel<T, RES, RNG><<<grid, kDropThreads, 0, ctx->stream>>>(o, x, r, n, rule);
                     }
+                } else {
+                    StridedArgs a{};
+                    const hmc_tensor_desc *d[3] = {out, src, residual};
+                    a.ndim = dims;
+                    a.n = n;
+                    for (int k = 0; k < 3; ++k) {
+                        a.base[k] = layer_base(d[k]);
+                        for (int j = 0; j < dims; ++j) {
+                            a.sizes[j] = src->sizes[j];
+                            a.strides[k][j] = d[k] != nullptr ? d[k]->strides[j] : 0;
+                        }
+                    }
+                    dropout_strided_kernel<T, RES, RNG><<<grid, kDropThreads, 0, ctx->stream>>>(a, rule);
                 }
-                if (residual != nullptr) dropout_strided_kernel<T, true><<<grid, kDropThreads, 0, ctx->stream>>>(a, rule);
-                else dropout_strided_kernel<T, false><<<grid, kDropThreads, 0, ctx->stream>>>(a, rule);
-            }
-            return launch_status("dropout kernel launch");
+                return launch_status("dropout kernel launch");
+            };
+            using Yes = std::true_type;
+            using No = std::false_type;
+            if (residual != nullptr) return none ? launch(Yes{}, No{}) : launch(Yes{}, Yes{});
+            return none ? launch(No{}, No{}) : launch(No{}, Yes{});
         });
     });
 }

@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
             const T *p = reinterpret_cast<const T *>(a.src) + sample * a.wsrc.n + (first + ty) * a.wsrc.s + channel;
             const int64_t step = t.ty * a.wsrc.s;
 #pragma unroll 4
-            for (int k = 0; k < have; ++k, p += step) copy_16(mine + k * kBlock, p);
+            for (int k = 0; k < have; ++k, p += step) async_copy_16(mine + k * kBlock, p);
             async_copy_commit();
         }
         const Columns<V> column(tile, tx, ty, t.ty);

@@ -114,10 +114,6 @@ template <class C, int V> __device__ __forceinline__ Memory carve(unsigned char 
     return m;
 }
 
-__device__ __forceinline__ void copy_16(void *shared_dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared_dst))), "l"(src) : "memory");
-}
-
 // A thread's place in the columns for its V channels: of channel i at[i], in group[i] of the tile.
 template <int V> struct Columns {
     int at[V], group[V];

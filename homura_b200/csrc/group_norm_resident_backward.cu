@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(kBlock, 2) resident_backward_kernel(const __gr
             const T *pd = reinterpret_cast<const T *>(a.dout) + sample * a.wdout.n + (first + ty) * a.wdout.s + channel;
             const int64_t x_step = t.ty * a.wsrc.s, d_step = t.ty * a.wdout.s;
             for (int k = 0; k < have; ++k, px += x_step, pd += d_step) {
-                copy_16(xs + k * kBlock, px);
-                copy_16(ds + k * kBlock, pd);
+                async_copy_16(xs + k * kBlock, px);
+                async_copy_16(ds + k * kBlock, pd);
             }
             async_copy_commit();
         }
