@@ -37,16 +37,19 @@ __device__ __forceinline__ typename Comp<T>::C drop(uint32_t word, T x, T residu
     }
 }
 
-// Eight neighbours from their two Philox blocks, the first of which is 2 * piece.
-template <class T, bool RES, bool RNG>
+// Eight neighbours from their two Philox blocks, the first of which is offset + 2 * piece. SAME: the upper half of all block
+// numbers is the one the keys were made for; then a block's first product is its neighbour's and a sum.
+template <class T, bool RES, bool RNG, bool SAME>
 __device__ __forceinline__ Pack<T, kPer> drop_piece(int64_t piece, const Pack<T, kPer> &x, const Pack<T, kPer> &r,
                                                     const DropRule<typename Comp<T>::C> &rule) {
     using C = typename Comp<T>::C;
     C v[kPer];
+    const uint64_t block = rule.offset + static_cast<uint64_t>(piece) * (kPer / 4);
+    const uint64_t product = static_cast<uint64_t>(kPhiloxM0) * static_cast<uint32_t>(block);
 #pragma unroll
     for (int b = 0; b < kPer / 4; ++b) {
         Words4 w{};
-        if constexpr (RNG) w = philox_block(rule.offset + static_cast<uint64_t>(piece) * (kPer / 4) + b, rule.keys);
+        if constexpr (RNG) w = SAME ? philox_block_same_high(product + static_cast<uint64_t>(b) * kPhiloxM0, rule.keys) : philox_block(block + b, rule.keys);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[4 * b + j] = drop<T, RES, RNG>(w.w[j], x.v[4 * b + j], r.v[4 * b + j], rule);
     }
@@ -61,7 +64,8 @@ __device__ __forceinline__ Pack<T, kPer> drop_piece(int64_t piece, const Pack<T,
     return y;
 }
 
-// What is left of a piece element by element: the last one, or all where an operand does not start on 16 bytes.
+// What is left of a piece element by element: the last one, or all where an operand does not start on 16 bytes or the block
+// numbers pass a multiple of 2^32.
 template <class T, bool RES, bool RNG>
 __device__ __forceinline__ void drop_ragged(T *out, const T *src, const T *residual, int64_t n, int64_t piece, const DropRule<typename Comp<T>::C> &rule) {
     Pack<T, kPer> x, r;
@@ -73,7 +77,7 @@ __device__ __forceinline__ void drop_ragged(T *out, const T *src, const T *resid
             if constexpr (RES) r.v[j] = residual[i0 + j];
         }
     }
-    const Pack<T, kPer> y = drop_piece<T, RES, RNG>(piece, x, r, rule);
+    const Pack<T, kPer> y = drop_piece<T, RES, RNG, false>(piece, x, r, rule);
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
         if (i0 + j < n) out[i0 + j] = y.v[j];
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kDropThreads) dropout_ragged_kernel(T *out, co
     }
 }
 
-// Contiguous operands on 16-byte boundaries: a resident grid walks the pieces, and a thread's next pieces come through a
+// Contiguous operands on 16-byte boundaries, block numbers that agree in their upper half: a resident grid walks the pieces, and a thread's next pieces come through a
 // ring in shared memory that its own asynchronous copies fill while it works out the present one's words: the rounds of the
 // generator and the memory's latency overlap without a register spent on data in flight.
 template <class T, bool RES> struct DropRing {
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(kDropThreads, sizeof(T) == 8 ? 2 : 4) dropout_
                 memcpy(reinterpret_cast<char *>(&x) + 16 * w, mine + stage * G::kPiece + w * (kDropThreads * 16), 16);
                 if constexpr (RES) memcpy(reinterpret_cast<char *>(&r) + 16 * w, mine + stage * G::kPiece + (G::kWords + w) * (kDropThreads * 16), 16);
             }
-            vector_store<T, kPer>(out + piece * kPer, drop_piece<T, RES, RNG>(piece, x, r, rule), false);
+            vector_store<T, kPer>(out + piece * kPer, drop_piece<T, RES, RNG, true>(piece, x, r, rule), false);
         } else {
             drop_ragged<T, RES, RNG>(out, src, residual, n, piece, rule);
         }
@@ -206,20 +210,22 @@ HMC_API hmc_status hmc_dropout(hmc_context_t ctx, const hmc_tensor_desc *out, co
         const bool is_flat = flat(out) && flat(src) && flat(residual);
         auto aligned = [&](const hmc_tensor_desc *d) { return reinterpret_cast<uintptr_t>(layer_base(d)) % 16 == 0; };
         const bool vectors = aligned(out) && aligned(src) && (residual == nullptr || aligned(residual));
+        const uint64_t last_block = offset + (static_cast<uint64_t>(n) - 1) / 4;
+        const bool same_high = last_block >> 32 == offset >> 32;
         const int64_t pieces = ceil_div(n, is_flat ? kPer : 4);
         const int64_t blocks = ceil_div(pieces, kDropThreads);
         const unsigned grid = static_cast<unsigned>(blocks < (int64_t{1} << 30) ? blocks : (int64_t{1} << 30));
         return dispatch_float(src->dtype, [&](auto tag) -> hmc_status {
             using T = decltype(tag);
             using C = typename Comp<T>::C;
-            const DropRule<C> rule{philox_keys(seed), offset, none ? 0u : (all ? 0xFFFFFFFFu : static_cast<uint32_t>(threshold) - 1u),
+            const DropRule<C> rule{philox_keys(seed, static_cast<uint32_t>(offset >> 32)), offset, none ? 0u : (all ? 0xFFFFFFFFu : static_cast<uint32_t>(threshold) - 1u),
                                    all ? C(0) : static_cast<C>(1.0 / (1.0 - p))};
             const auto launch = [&](auto with_residual, auto with_words) -> hmc_status {
                 constexpr bool RES = decltype(with_residual)::value, RNG = decltype(with_words)::value;
                 if (is_flat) {
                     T *o = reinterpret_cast<T *>(layer_base(out));
                     const T *x = reinterpret_cast<const T *>(layer_base(src)), *r = reinterpret_cast<const T *>(layer_base(residual));
-                    if (vectors) {
+                    if (vectors && same_high) {
                         using G = DropRing<T, RES>;
                         static bool raised[kDropDevices] = {};  // (a race between threads only repeats the call)
                         if (G::kBytes > 32768 && (ctx->device >= kDropDevices || !raised[ctx->device])) {

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 import weakref
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
@@ -899,7 +900,11 @@ class CudaBackend:
         if out.numel == 0 or any(t.shape != out.shape for t in operands):
             d = [plain_desc(kernel, t) for t in operands]  # nothing to write, or refused by the library
         elif all(t.is_contiguous() for t in operands):
-            d = [_flat_desc(t) for t in operands]
+            n, step = (out.numel,), (1,)
+            if CHECK_REACH:
+                for t in operands:
+                    check_reach(kernel, t, t.offset, [(n[0], [1])], 0)
+            d = [packed_desc(t, n, step) for t in operands]
         else:
             d = descs(kernel, operands)
         self._check(self.lib.hmc_dropout(self.ctx, d[0], d[1], d[2] if len(d) > 2 else None, float(p), *state))
@@ -979,11 +984,18 @@ def plain_desc(kernel: str, t: Optional[TensorData]) -> Optional[hmc_tensor_desc
         raise BackendError(ffi.HMC_INVALID, f"{kernel} on CUDA supports at most {MAX_DIMS} dimensions, got {n}")
     if CHECK_REACH:
         check_reach(kernel, t, t.offset, [(size, [st]) for size, st in zip(t.shape, t.strides)], 0)
-    d = hmc_tensor_desc()
-    d.data, d.offset, d.dtype, d.ndim = t.storage.address, t.offset, t.dtype, n
-    d.sizes[:n] = t.shape
-    d.strides[:n] = t.strides
-    return d
+    return packed_desc(t, t.shape, t.strides)
+
+
+# A description packed in one go: a third of the time of setting its fields one by one, of which a small kernel's call has
+# as many as it has operands.
+_PACK_DESC = [struct.Struct(f"<Qqii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x") for n in range(MAX_DIMS + 1)]
+assert all(s.size == ctypes.sizeof(hmc_tensor_desc) for s in _PACK_DESC)
+
+
+def packed_desc(t: TensorData, shape: Sequence[int], strides: Sequence[int]) -> hmc_tensor_desc:
+    n = len(shape)
+    return hmc_tensor_desc.from_buffer_copy(_PACK_DESC[n].pack(t.storage.address, t.offset, t.dtype, n, *shape, *strides))
 
 
 def channels_last_desc(kernel: str, t: TensorData) -> hmc_tensor_desc:
