@@ -7,7 +7,7 @@ namespace gnorm {
 namespace {
 
 template <class T, int V, int K, bool WIDE, int ACT>
-__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : (V > 1 && K * V <= 8 ? 3 : 2)) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || K == 16 ? 1 : (V > 1 && K * V <= 8 ? 3 : 2)) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
     using C = typename Comp<T>::C;
     constexpr int U = samples_at_a_time(K);
     constexpr bool kKeep = K * V <= 16;  // parameters in registers

@@ -14,7 +14,7 @@ namespace hmc {
 namespace gnorm {
 
 // A lane's vectors at most: 32 values forward, 16 backward, where the sums for dweight and dbias stand beside them.
-constexpr int most_vectors(int v, bool backward) { return (backward ? 16 : 32) / v < 8 ? (backward ? 16 : 32) / v : 8; }
+constexpr int most_vectors(int v, bool backward) { return v == 1 ? 16 : ((backward ? 16 : 32) / v < 8 ? (backward ? 16 : 32) / v : 8); }
 
 struct Teams {
     int32_t lanes;            // lanes a team
@@ -203,15 +203,17 @@ hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation,
 // positions == 1
 hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation, const RowsBackwardArgs &a, int64_t row_blocks);
 
-// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (8 only without vectors, 2 at least for a block).
+// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (4 and 16 without
+// vectors, 2 at least for a block).
 template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(const Teams &t, F &&f) {
     constexpr int V = kVector<T>, kMost = most_vectors(V, BACKWARD);
     const auto with = [&](auto v, auto k, auto wide) { return f(v, k, wide); };
     using One = std::integral_constant<int, 1>;
     using Vec = std::integral_constant<int, V>;
     if (t.v == 1) {
-        if (t.wide) return with(One{}, std::integral_constant<int, 8>{}, std::true_type{});
-        return with(One{}, std::integral_constant<int, 8>{}, std::false_type{});
+        if (t.wide) return with(One{}, std::integral_constant<int, 16>{}, std::true_type{});
+        if (t.k <= 4) return with(One{}, std::integral_constant<int, 4>{}, std::false_type{});
+        return with(One{}, std::integral_constant<int, 16>{}, std::false_type{});
     }
     if (t.wide) {
         if (t.k <= 2) return with(Vec{}, std::integral_constant<int, 2>{}, std::true_type{});

@@ -11,7 +11,8 @@ struct ForwardArgs {
     const char *initial;  // null: zeros
     char *last;           // null: not wanted
     Walk wout, wgate, wx, winitial, wlast;
-    int64_t time, channels, tiles, items;
+    int64_t time, channels;
+    Columns columns;
     int32_t warps_time;
     int *status;
 };
@@ -35,14 +36,13 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
     begin_exchange(shared, p);
     uint32_t rounds = 0;
     bool gave_up = false;
-    for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
-        const int64_t batch = item / a.tiles;
-        const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
-        const int64_t channel = tile + p.slot;
-        const bool live = channel < a.channels;
+    for (int64_t item = blockIdx.x / p.cluster; item < a.columns.items; item += gridDim.x / p.cluster) {
+        const Column at_column = column_of<V>(a.columns, item, a.warps_time, p.wc, p.lane);
+        const int64_t batch = at_column.batch, channel = at_column.channel;
+        const bool live = at_column.live;
         // what this lane loads or copies: its own channels, or its part of a row
-        const int64_t column = COPY > 0 ? tile + G::channel() : channel;
-        const bool loads = column < a.channels;
+        const int64_t column = COPY == 16 ? at_column.tile + G::channel() : channel;
+        const bool loads = COPY == 16 ? column < a.channels : live;
         const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + column * a.wgate.c;
         const T *x = reinterpret_cast<const T *>(a.x) + batch * a.wx.b + column * a.wx.c;
         T *out = reinterpret_cast<T *>(a.out) + batch * a.wout.b + channel * a.wout.c;
@@ -170,9 +170,8 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
 
 template <class T, int V, int R, int COPY>
 hmc_status launch_forward(hmc_context_t ctx, ForwardArgs &a, int64_t batch, int32_t flags) {
-    const Shape shape = plan_launch(batch, a.time, a.channels, V, R, per_sm<T>(R));
-    a.tiles = shape.tiles;
-    a.items = shape.items;
+    const bool flat = COPY != 16 && flat_columns(a.channels, V);
+    const Shape shape = plan_launch(batch, a.time, a.channels, flat, V, R, per_sm<T>(R), &a.columns);
     a.warps_time = shape.warps_time;
     constexpr int kShared = COPY > 0 ? kWarps * kStages * 2 * R * Ring<T, V, COPY>::kRow : 0;
     const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
@@ -230,12 +229,15 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
                 if (!pairs) return time == 1 ? launch_forward<T, 1, 1, 0>(ctx, a, batch, flags) : launch_forward<T, 1, 8, 0>(ctx, a, batch, flags);
             }
             if (time == 1) return launch_forward<T, V, 1, 0>(ctx, a, batch, flags);
+            const bool flat = flat_columns(channels, V), lines = wide && !flat;
             if constexpr (sizeof(T) < 8) {
                 // Sixteen rows a lane halve the exchanges, two blocks an SM then: where that many blocks take all channels.
-                const bool few = batch * ceil_div(channels, int64_t{32} * V) <= int64_t{148} * 2 * kWarps;
-                if (few) return wide ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);
+                const int64_t warps = flat ? ceil_div(batch * channels, int64_t{32} * V) : batch * ceil_div(channels, int64_t{32} * V);
+                if (warps <= int64_t{148} * 2 * kWarps) {
+                    return lines ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);
+                }
             }
-            return wide ? launch_forward<T, V, 8, 16>(ctx, a, batch, flags) : launch_forward<T, V, 8, kWord>(ctx, a, batch, flags);
+            return lines ? launch_forward<T, V, 8, 16>(ctx, a, batch, flags) : launch_forward<T, V, 8, kWord>(ctx, a, batch, flags);
         });
     });
 }

@@ -204,6 +204,35 @@ __device__ __forceinline__ void copy_rows(unsigned char *ring, int to, const T *
     }
 }
 
+// The columns (batch, V channels) of an item. `flat`: lanes take the columns of all batches one after another, so that few
+// channels, or a number that no warp divides, leave no lane idle; every lane then has a batch of its own, and copies are of
+// its own word. Otherwise a warp's columns lie side by side in one batch.
+struct Columns {
+    int64_t channels, tiles, items;
+    int64_t per_batch, all;  // flat: columns of a batch and of all batches
+    int32_t flat;
+};
+struct Column {
+    int64_t batch, channel, tile;  // tile: the warp's first channel (not flat)
+    bool live;
+};
+template <int V> __device__ __forceinline__ Column column_of(const Columns &c, int64_t item, int warps_time, int wc, int lane) {
+    Column r;
+    if (c.flat) {
+        const int64_t column = (item * (kWarps / warps_time) + wc) * 32 + lane;
+        r.live = column < c.all;
+        r.batch = r.live ? column / c.per_batch : 0;
+        r.channel = r.live ? (column - r.batch * c.per_batch) * V : 0;
+        r.tile = 0;
+    } else {
+        r.batch = item / c.tiles;
+        r.tile = ((item - r.batch * c.tiles) * (kWarps / warps_time) + wc) * (32 * V);
+        r.channel = r.tile + lane * V;
+        r.live = r.channel < c.channels;
+    }
+    return r;
+}
+
 // What a launch looks like; see plan_launch.
 struct Shape {
     int32_t warps_time;  // WT
@@ -216,7 +245,12 @@ struct Shape {
 // WT and the cluster grow while every block still finds a place at once, `per_sm` on an SM, and the time axis feeds them:
 // a second, partly filled wave costs more than the warps it brings. The constant is B200's SM count, not the device's, so
 // that the order of folding is the same everywhere.
-inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, int v, int rows, int per_sm) {
+inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, bool flat, int v, int rows, int per_sm, Columns *columns) {
+    *columns = Columns{channels, 0, 0, channels / v, batch * (channels / v), flat ? 1 : 0};
+    if (flat) {
+        channels *= batch;
+        batch = 1;
+    }
     const int64_t places = int64_t{148} * per_sm;
     Shape s{1, 1, 0, 0, 0};
     const int64_t warps = batch * ceil_div(channels, int64_t{32} * v);  // (both counts are below 2^62 / (32 v))
@@ -229,6 +263,8 @@ inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, int v, i
     }
     s.tiles = ceil_div(channels, int64_t{32} * v * (kWarps / s.warps_time));
     s.items = batch * s.tiles;
+    columns->tiles = s.tiles;
+    columns->items = s.items;
     const int64_t most = (int64_t{1} << 30) / s.cluster;
     s.grid = static_cast<unsigned>((s.items < most ? s.items : most) * s.cluster);
     return s;
@@ -267,6 +303,9 @@ template <class P> inline Walk walk_rows(const hmc_tensor_desc *d, bool backward
     return w;
 }
 inline Walk walk_state(const hmc_tensor_desc *d) { return d == nullptr ? Walk{0, 0, 0} : Walk{d->strides[0], 0, d->strides[1]}; }
+
+// Whether the columns of all batches are laid out flat: where warps within one batch would leave a fifth of their lanes idle.
+inline bool flat_columns(int64_t channels, int v) { return ceil_div(channels, int64_t{32} * v) * 32 * v * 4 > channels * 5; }
 
 template <class F> hmc_status dispatch_flags(int32_t flags, F &&f) {
     using Yes = std::true_type;

@@ -14,7 +14,8 @@ struct BackwardArgs {
     const char *gate, *x, *out, *dout;          // x: read with COMP only
     const char *initial, *dlast;                // null: zeros
     Walk wdgate, wdx, wdinitial, wgate, wx, wout, wdout, winitial, wdlast;
-    int64_t time, channels, tiles, items;
+    int64_t time, channels;
+    Columns columns;
     int32_t warps_time;
     int *status;
 };
@@ -39,14 +40,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
     begin_exchange(shared, p);
     uint32_t rounds = 0;
     bool gave_up = false;
-    for (int64_t item = blockIdx.x / p.cluster; item < a.items; item += gridDim.x / p.cluster) {
-        const int64_t batch = item / a.tiles;
-        const int64_t tile = ((item - batch * a.tiles) * (kWarps / a.warps_time) + p.wc) * (32 * V);  // the warp's first channel
-        const int64_t channel = tile + p.slot;
-        const bool live = channel < a.channels;
+    for (int64_t item = blockIdx.x / p.cluster; item < a.columns.items; item += gridDim.x / p.cluster) {
+        const Column at_column = column_of<V>(a.columns, item, a.warps_time, p.wc, p.lane);
+        const int64_t batch = at_column.batch, channel = at_column.channel;
+        const bool live = at_column.live;
         // what this lane loads or copies: its own channels, or its part of a row
-        const int64_t column = COPY > 0 ? tile + G::channel() : channel;
-        const bool loads = column < a.channels;
+        const int64_t column = COPY == 16 ? at_column.tile + G::channel() : channel;
+        const bool loads = COPY == 16 ? column < a.channels : live;
         const T *gate = reinterpret_cast<const T *>(a.gate) + batch * a.wgate.b + column * a.wgate.c;
         const T *x = COMP ? reinterpret_cast<const T *>(a.x) + batch * a.wx.b + column * a.wx.c : nullptr;
         const T *out = reinterpret_cast<const T *>(a.out) + batch * a.wout.b + column * a.wout.c;
@@ -199,9 +199,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
 
 template <class T, int V, int R, int COPY>
 hmc_status launch_backward(hmc_context_t ctx, BackwardArgs &a, int64_t batch, int32_t flags) {
-    const Shape shape = plan_launch(batch, a.time, a.channels, V, R, kPerSm<T>);
-    a.tiles = shape.tiles;
-    a.items = shape.items;
+    const bool flat = COPY != 16 && flat_columns(a.channels, V);
+    const Shape shape = plan_launch(batch, a.time, a.channels, flat, V, R, kPerSm<T>, &a.columns);
     a.warps_time = shape.warps_time;
     const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
         static bool raised[kKnownDevices] = {};
@@ -277,7 +276,7 @@ HMC_API hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_t
                 if (!pairs) return time == 1 ? launch_backward<T, 1, 1, 0>(ctx, a, batch, flags) : launch_backward<T, 1, 8, 0>(ctx, a, batch, flags);
             }
             if (time == 1) return launch_backward<T, V, 1, 0>(ctx, a, batch, flags);
-            return wide ? launch_backward<T, V, 8, 16>(ctx, a, batch, flags) : launch_backward<T, V, 8, kWord>(ctx, a, batch, flags);
+            return wide && !flat_columns(channels, V) ? launch_backward<T, V, 8, 16>(ctx, a, batch, flags) : launch_backward<T, V, 8, kWord>(ctx, a, batch, flags);
         });
     });
 }
