@@ -3,6 +3,8 @@
 // Three steps: every block takes the moments of its run of rows (held in registers: the mean first, then the squares of
 // the deviations from it, run by run merged pairwise), a small kernel merges the pieces of each group, and an elementwise
 // pass normalises. Where one block holds a whole group the middle step falls away.
+#include <algorithm>
+
 #include "group_norm_resident.cuh"
 
 namespace hmc {
@@ -205,9 +207,12 @@ struct Plan {
     Cut moments, apply;
     int64_t pieces_bytes, bytes;
 };
-Plan make_plan(const Problem &p, bool vectors) {
+Plan make_plan(const Problem &p, Align align) {
     Plan r{};
-    r.t = make_tiling(p.channels, p.groups, 16 / element_size(p.dtype), vectors);
+    const int es = element_size(p.dtype);
+    r.t = make_tiling(p.channels, p.groups, align == Align::kLine ? 16 / es : narrow_vector(es), align != Align::kAny);
+    // (a tiling by lines that does not come out is one by single values; by words it may)
+    if (align == Align::kLine && r.t.v == 1) r.t = make_tiling(p.channels, p.groups, narrow_vector(es), true);
     r.moments = cut_rows(p, r.t, static_cast<int64_t>(r.t.ty) * kRows);
     r.apply = cut_rows(p, r.t, r.t.ty);
     const int64_t pieces = r.moments.chunks * r.t.segments;
@@ -220,13 +225,15 @@ Plan make_plan(const Problem &p, bool vectors) {
 
 // What the forward pass needs whatever the alignment of its operands.
 int64_t forward_workspace(const Problem &p) {
-    const int vector = 16 / element_size(p.dtype);
-    const auto need = [&](bool vectors) -> int64_t {
-        if (make_teams(p, vector, vectors, false).v > 0 || make_resident(p, vector, vectors, 1).t.v > 0) return 0;
-        return make_plan(p, vectors).bytes;
+    const int es = element_size(p.dtype), vector = 16 / es;
+    const auto need = [&](Align align) -> int64_t {
+        if (make_teams(p, vector, align == Align::kLine, false).v > 0 || find_resident(p, align, 1).t.v > 0) return 0;
+        return make_plan(p, align).bytes;
     };
-    const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
-    return a > b ? a : b;
+    int64_t most = es >= 4 ? 0 : need(Align::kAny);
+    if (p.channels * es % 4 == 0) most = std::max(most, need(Align::kWord));
+    if (p.channels % vector == 0) most = std::max(most, need(Align::kLine));
+    return most;
 }
 
 }  // namespace gnorm
@@ -259,8 +266,8 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
         s = check_workspace(forward_workspace(p), workspace, workspace_bytes);
         if (s != HMC_OK) return s;
         HMC_ENTER(ctx);
-        const bool vectors = all_vectors(src, out);
-        const Teams teams = make_teams(p, 16 / element_size(p.dtype), vectors, false);
+        const Align align = alignment(p.dtype, src, out);
+        const Teams teams = make_teams(p, 16 / element_size(p.dtype), align == Align::kLine, false);
         if (teams.v > 0) {
             RowsForwardArgs r{};
             r.out = layer_base(out);
@@ -283,7 +290,7 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
             r.eps = eps;
             return launch_rows_forward(ctx, p.dtype, activation, r);
         }
-        const Resident resident = make_resident(p, 16 / element_size(p.dtype), vectors, 1);
+        const Resident resident = find_resident(p, align, 1);
         if (resident.t.v > 0) {
             ResidentForwardArgs r{};
             r.out = layer_base(out);
@@ -305,7 +312,7 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
             r.eps = eps;
             return launch_resident_forward(ctx, p.dtype, activation, r);
         }
-        const Plan plan = make_plan(p, vectors);
+        const Plan plan = make_plan(p, align);
         StatArgs st{};
         st.src = layer_base(src);
         st.wsrc = Rows{src->strides[0], src->strides[1]};
@@ -353,6 +360,9 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
                 });
             };
             if (plan.t.v == kVector<T>) return run(std::integral_constant<int, kVector<T>>{});
+            if constexpr (sizeof(T) == 2) {
+                if (plan.t.v == 2) return run(std::integral_constant<int, 2>{});
+            }
             return run(std::integral_constant<int, 1>{});
         });
     });

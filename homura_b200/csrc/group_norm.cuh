@@ -284,8 +284,13 @@ template <class F> inline hmc_status dispatch_activation(int32_t activation, F &
         default: return f(std::integral_constant<int, HMC_ACTIVATION_NONE>{});
     }
 }
-// Vectors of 16 bytes along the channels of every operand.
-template <class... D> inline bool all_vectors(const D *...d) { return (layer_vectors(d, 16) && ...); }
+// How regular the operands are: vectors of 16 bytes, words of 4, or neither.
+enum class Align { kAny, kWord, kLine };
+template <class... D> inline Align alignment(int dtype, const D *...d) {
+    if ((layer_vectors(d, 16) && ...)) return Align::kLine;
+    return element_size(dtype) >= 4 || (layer_vectors(d, 4) && ...) ? Align::kWord : Align::kAny;
+}
+constexpr int narrow_vector(int es) { return es == 2 ? 2 : 1; }  // elements of a word
 template <class T> constexpr int kVector = 16 / static_cast<int>(sizeof(T));
 
 inline unsigned grid_for(int64_t blocks) { return static_cast<unsigned>(blocks < (int64_t{1} << 30) ? blocks : (int64_t{1} << 30)); }

@@ -3,6 +3,8 @@
 // Three steps: sums over each run of rows of dz and dz * xhat (by channel for weight and bias, by group, weighted, for
 // the input), a small kernel that folds the runs in order, and an elementwise pass. Channel sums are kept in f64 across
 // the runs a block takes, and folded over the blocks in f64.
+#include <algorithm>
+
 #include "group_norm_resident.cuh"
 
 namespace hmc {
@@ -224,17 +226,20 @@ struct Plan {
     int64_t columns;
     int64_t pieces_bytes, means_bytes, bytes;
 };
-Plan make_plan(const Problem &p, bool vectors) {
+Plan make_plan(const Problem &p, Align align) {
     Plan r{};
-    r.t = make_tiling(p.channels, p.groups, 16 / element_size(p.dtype), vectors);
+    const int es = element_size(p.dtype);
+    r.t = make_tiling(p.channels, p.groups, align == Align::kLine ? 16 / es : narrow_vector(es), align != Align::kAny);
+    // (a tiling by lines that does not come out is one by single values; by words it may)
+    if (align == Align::kLine && r.t.v == 1) r.t = make_tiling(p.channels, p.groups, narrow_vector(es), true);
     r.sums = cut_rows(p, r.t, static_cast<int64_t>(r.t.ty) * 4);
     r.apply = cut_rows(p, r.t, r.t.ty);
     const int64_t pairs = p.samples * r.sums.chunks;
     r.columns = ceil_div(kBlocksWanted, r.t.tiles);
     if (r.columns > pairs) r.columns = pairs;
-    const int64_t pieces = r.sums.chunks * r.t.segments, es = element_size(p.stat_dtype);
-    r.pieces_bytes = pieces == 1 ? 0 : ceil_div(p.samples * p.groups * pieces * 2 * es, 16) * 16;
-    r.means_bytes = ceil_div(p.samples * p.groups * 2 * es, 16) * 16;
+    const int64_t pieces = r.sums.chunks * r.t.segments, wide = element_size(p.stat_dtype);
+    r.pieces_bytes = pieces == 1 ? 0 : ceil_div(p.samples * p.groups * pieces * 2 * wide, 16) * 16;
+    r.means_bytes = ceil_div(p.samples * p.groups * 2 * wide, 16) * 16;
     r.bytes = r.pieces_bytes + r.means_bytes + r.columns * 2 * p.channels * 8;
     return r;
 }
@@ -246,7 +251,6 @@ struct RowRuns {
 };
 RowRuns make_runs(const Problem &p, int vector, bool vectors) {
     RowRuns r{};
-    if (p.positions != 1) return r;
     r.t = make_teams(p, vector, vectors, true);
     if (r.t.v == 0) return r;
     const int64_t rounds = ceil_div(p.samples, r.t.samples_at_once);
@@ -258,7 +262,7 @@ RowRuns make_runs(const Problem &p, int vector, bool vectors) {
     }
     r.run = run;
     r.row_blocks = ceil_div(rounds, run);
-    r.partials = r.row_blocks * r.t.samples_at_once;
+    r.partials = r.row_blocks * r.t.samples_at_once * p.positions;
     r.bytes = ceil_div(r.partials * 2 * p.channels * element_size(p.stat_dtype), 16) * 16;
     return r;
 }
@@ -275,15 +279,20 @@ int64_t resident_columns(const Problem &p, const Resident &r) {
 }  // namespace
 
 int64_t backward_workspace(const Problem &p) {
-    const int vector = 16 / element_size(p.dtype);
-    const auto need = [&](bool vectors) -> int64_t {
-        const RowRuns r = make_runs(p, vector, vectors);
+    const int es = element_size(p.dtype), vector = 16 / es;
+    const auto need = [&](Align align) -> int64_t {
+        const RowRuns r = make_runs(p, vector, align == Align::kLine);
         if (r.t.v > 0) return r.bytes;
-        const Resident resident = make_resident(p, vector, vectors, 2);
-        return resident.t.v > 0 ? ceil_div(resident_columns(p, resident) * resident.cluster * 2 * p.channels * element_size(p.stat_dtype), 16) * 16 : make_plan(p, vectors).bytes;
+        const Resident resident = find_resident(p, align, 2);
+        if (resident.t.v > 0) {
+            return ceil_div(resident_columns(p, resident) * resident.cluster * 2 * p.channels * element_size(p.stat_dtype), 16) * 16;
+        }
+        return make_plan(p, align).bytes;
     };
-    const int64_t a = need(false), b = p.channels % vector == 0 ? need(true) : 0;
-    return a > b ? a : b;
+    int64_t most = es >= 4 ? 0 : need(Align::kAny);
+    if (p.channels * es % 4 == 0) most = std::max(most, need(Align::kWord));
+    if (p.channels % vector == 0) most = std::max(most, need(Align::kLine));
+    return most;
 }
 int64_t forward_workspace(const Problem &p);
 
@@ -361,10 +370,10 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
                 return launch_status("group norm channel kernel launch");
             });
         }
-        const bool vectors = all_vectors(src, dout, dsrc);
-        const RowRuns rows = make_runs(p, 16 / element_size(p.dtype), vectors);
-        const Resident resident = rows.t.v > 0 ? Resident{} : make_resident(p, 16 / element_size(p.dtype), vectors, 2);
-        const Plan plan = rows.t.v > 0 || resident.t.v > 0 ? Plan{} : make_plan(p, vectors);
+        const Align align = alignment(p.dtype, src, dout, dsrc);
+        const RowRuns rows = make_runs(p, 16 / element_size(p.dtype), align == Align::kLine);
+        const Resident resident = rows.t.v > 0 ? Resident{} : find_resident(p, align, 2);
+        const Plan plan = rows.t.v > 0 || resident.t.v > 0 ? Plan{} : make_plan(p, align);
         a.src = layer_base(src);
         a.dout = layer_base(dout);
         a.mean = layer_base(mean);
@@ -403,6 +412,7 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
             b.groups = p.groups;
             b.cg = p.channels / p.groups;
             b.channels = p.channels;
+            b.positions = p.positions;
             b.run = rows.run;
             b.affine = affine;
             b.by_channel = sums_wanted ? workspace : nullptr;
@@ -466,6 +476,9 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
                 });
             };
             if (plan.t.v == kVector<T>) return run(std::integral_constant<int, kVector<T>>{});
+            if constexpr (sizeof(T) == 2) {
+                if (plan.t.v == 2) return run(std::integral_constant<int, 2>{});
+            }
             return run(std::integral_constant<int, 1>{});
         });
     });

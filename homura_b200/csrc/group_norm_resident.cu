@@ -5,10 +5,10 @@ namespace hmc {
 namespace gnorm {
 namespace {
 
-template <class T, int ACT>
+template <class T, int V, int ACT>
 __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_constant__ ResidentForwardArgs a) {
     using C = typename Comp<T>::C;
-    constexpr int V = kVector<T>;
+    constexpr int kBytes = V * static_cast<int>(sizeof(T));
     extern __shared__ __align__(16) unsigned char memory[];
     const Memory m = carve<C, V>(memory, a.r, 1);
     const Tiling &t = a.r.t;
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
             const T *p = reinterpret_cast<const T *>(a.src) + sample * a.wsrc.n + (first + ty) * a.wsrc.s + channel;
             const int64_t step = t.ty * a.wsrc.s;
 #pragma unroll 4
-            for (int k = 0; k < have; ++k, p += step) async_copy_16(mine + k * kBlock, p);
+            for (int k = 0; k < have; ++k, p += step) copy_async<kBytes>(mine + k * kBlock, p);
             async_copy_commit();
         }
         const Columns<V> column(tile, tx, ty, t.ty);
@@ -163,11 +163,14 @@ hmc_status launch_resident_forward(hmc_context_t ctx, int dtype, int32_t activat
     return dispatch_float(dtype, [&](auto tag) -> hmc_status {
         using T = decltype(tag);
         return dispatch_activation(activation, [&](auto act) -> hmc_status {
-            static bool raised[kRowDevices] = {};
             const int64_t units = a.samples * a.r.t.tiles;
             const int64_t most = (int64_t{1} << 30) / a.r.cluster;
-            return launch_resident(ctx, resident_kernel<T, decltype(act)::value>, raised, units < most ? units : most, a.r, a,
-                                   "group norm kernel launch");
+            if (a.r.t.v == kVector<T>) {
+                static bool raised[kRowDevices] = {};
+                return launch_resident(ctx, resident_kernel<T, kVector<T>, decltype(act)::value>, raised, units < most ? units : most, a.r, a, "group norm kernel launch");
+            }
+            static bool raised[kRowDevices] = {};
+            return launch_resident(ctx, resident_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, raised, units < most ? units : most, a.r, a, "group norm kernel launch");
         });
     });
 }

@@ -2,7 +2,8 @@
 // and written once.
 //
 // The positions of one sample are divided among the blocks of a cluster (one to eight). A thread copies its own column of
-// 16-byte vectors into shared memory asynchronously and reads only what it copied. What a thread finds for its
+// 16-byte vectors (of words of 4 bytes where rows or groups are not that regular, 8 for F64) into shared memory
+// asynchronously and reads only what it copied. What a thread finds for its
 // channels (over at most 64 rows at a time in the computation type) is laid out by group in shared memory, summed by a warp a
 // group in f64, and goes to the other blocks through distributed shared memory, where every block folds it in rank order.
 // That is one exchange a sample, whatever the direction.
@@ -32,9 +33,9 @@ struct Resident {
 
 // `operands` tensors are kept. Tiles are made wide enough for whole 128-byte lines where the groups allow, and, where
 // there are few positions, as wide as gives a block some tens of KB of work.
-inline Resident make_resident(const Problem &p, int vector, bool vectors, int operands) {
+inline Resident make_resident(const Problem &p, int vector, int operands) {
     Resident r{};
-    if (!vectors || p.positions < 2 || p.positions > (int64_t{1} << 20)) return r;
+    if (p.channels % vector != 0 || p.positions < 2 || p.positions > (int64_t{1} << 20)) return r;
     // (forward, squares are summed in f64, which leaves nothing to spare for F64's own moments: their pieces are merged pairwise)
     if (operands == 1 && p.dtype == HMC_F64) return r;
     const int es = element_size(p.dtype);
@@ -54,8 +55,8 @@ inline Resident make_resident(const Problem &p, int vector, bool vectors, int op
         s.t.ty = kBlock / s.t.tx;
         s.cluster = cluster;
         s.run = ceil_div(p.positions, cluster);
-        const int64_t slots = ceil_div(s.run, s.t.ty), data = slots * kBlock * 16;
-        const int64_t rest = kBlock * (es == 2 ? 64 : 32) + 2 * cluster * per * 16 + per * 16 + 64;
+        const int64_t slots = ceil_div(s.run, s.t.ty), data = ceil_div(slots * kBlock * vector * es, 16) * 16;
+        const int64_t rest = kBlock * vector * 2 * (es == 8 ? 8 : 4) + 2 * cluster * per * 16 + per * 16 + 64;
         if (data * operands + rest > kResidentShared) {
             s.t.v = 0;
             return s;
@@ -81,12 +82,13 @@ inline Resident make_resident(const Problem &p, int vector, bool vectors, int op
             }
         }
     } else {
-        for (int64_t width = line < widest ? line : widest;; width = unit) {
+        for (int64_t width = line < widest ? line : widest;;) {
             for (int cluster = 1; cluster <= kResidentCluster; cluster *= 2) {
                 r = shape(width, cluster);
                 if (r.t.v > 0 && r.shared <= kResidentWanted) break;
             }
-            if (r.t.v > 0 || width == unit) break;
+            if (r.t.v > 0 || width <= unit) break;
+            width = width / 2 / unit * unit < unit ? unit : width / 2 / unit * unit;  // (then rows of less than a line)
         }
         if (r.t.v == 0) return r;
     }
@@ -99,8 +101,18 @@ inline Resident make_resident(const Problem &p, int vector, bool vectors, int op
     return r;
 }
 
+inline Resident find_resident(const Problem &p, Align align, int operands) {
+    const int es = element_size(p.dtype);
+    if (align == Align::kLine) {
+        const Resident r = make_resident(p, 16 / es, operands);
+        if (r.t.v > 0) return r;
+    }
+    if (align != Align::kAny) return make_resident(p, narrow_vector(es), operands);
+    return Resident{};
+}
+
 struct Memory {  // a block's dynamic shared memory
-    unsigned char *data;   // [operands][slots][kBlock] vectors
+    unsigned char *data;   // [operands][slots][kBlock] vectors (or words)
     void *columns;         // Two<C> [groups of the tile][rows at a time * channels of a group]: what the threads found
     Two<double> *slots;    // [2][cluster][groups of the tile]
     Two<double> *folded;   // [groups of the tile]
@@ -112,6 +124,11 @@ template <class C, int V> __device__ __forceinline__ Memory carve(unsigned char 
     m.slots = reinterpret_cast<Two<double> *>(static_cast<unsigned char *>(m.columns) + kBlock * V * sizeof(Two<C>));
     m.folded = m.slots + 2 * r.cluster * r.t.groups_per_tile;
     return m;
+}
+
+template <int BYTES> __device__ __forceinline__ void copy_async(void *shared_dst, const void *src) {
+    if constexpr (BYTES == 16) async_copy_16(shared_dst, src);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared_dst))), "l"(src), "n"(BYTES) : "memory");
 }
 
 // A thread's place in the columns for its V channels: of channel i at[i], in group[i] of the tile.

@@ -7,10 +7,10 @@ namespace hmc {
 namespace gnorm {
 namespace {
 
-template <class T, int ACT>
+template <class T, int V, int ACT>
 __global__ void __launch_bounds__(kBlock, 2) resident_backward_kernel(const __grid_constant__ ResidentBackwardArgs a) {
     using C = typename Comp<T>::C;
-    constexpr int V = kVector<T>;
+    constexpr int kBytes = V * static_cast<int>(sizeof(T));
     extern __shared__ __align__(16) unsigned char memory[];
     const Memory m = carve<C, V>(memory, a.r, 2);
     const Tiling &t = a.r.t;
@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(kBlock, 2) resident_backward_kernel(const __gr
             const T *pd = reinterpret_cast<const T *>(a.dout) + sample * a.wdout.n + (first + ty) * a.wdout.s + channel;
             const int64_t x_step = t.ty * a.wsrc.s, d_step = t.ty * a.wdout.s;
             for (int k = 0; k < have; ++k, px += x_step, pd += d_step) {
-                async_copy_16(xs + k * kBlock, px);
-                async_copy_16(ds + k * kBlock, pd);
+                copy_async<kBytes>(xs + k * kBlock, px);
+                copy_async<kBytes>(ds + k * kBlock, pd);
             }
             async_copy_commit();
         }
@@ -141,9 +141,12 @@ hmc_status launch_resident_backward(hmc_context_t ctx, int dtype, int32_t activa
     return dispatch_float(dtype, [&](auto tag) -> hmc_status {
         using T = decltype(tag);
         return dispatch_activation(activation, [&](auto act) -> hmc_status {
+            if (a.r.t.v == kVector<T>) {
+                static bool raised[kRowDevices] = {};
+                return launch_resident(ctx, resident_backward_kernel<T, kVector<T>, decltype(act)::value>, raised, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
+            }
             static bool raised[kRowDevices] = {};
-            return launch_resident(ctx, resident_backward_kernel<T, decltype(act)::value>, raised, a.columns * a.r.t.tiles, a.r, a,
-                                   "group norm gradient kernel launch");
+            return launch_resident(ctx, resident_backward_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, raised, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
         });
     });
 }

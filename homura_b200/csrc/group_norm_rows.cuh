@@ -39,7 +39,17 @@ inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backwar
     t.v = v;
     t.vectors = static_cast<int32_t>(p.positions * (cg / v));
     t.row_vectors = static_cast<int32_t>(cg / v);
+    // Single values of several rows are read in small pieces, at some 150 GB/s; a cluster reads them side by side but spends
+    // about 4 us a sample on two blocks an SM, which only samples of about 2 KB (all operands) do not repay.
+    if (v == 1 && p.positions > 1 && p.positions * p.channels * element_size(p.dtype) * (backward ? 3 : 2) > 2048) {
+        t.v = 0;
+        return t;
+    }
     if (t.vectors > 32 * most_k) {
+        if (p.positions > 1) {  // the tiled kernels read several rows of wide groups side by side
+            t.v = 0;
+            return t;
+        }
         t.wide = true;
         t.lanes = kBlock;
         t.k = (t.vectors + kBlock - 1) / kBlock;
@@ -192,19 +202,18 @@ struct RowsBackwardArgs {
     Rows wdsrc, wsrc, wdout;
     int64_t mean_n, mean_g, rstd_n, rstd_g;
     Teams t;
-    int64_t samples, groups, cg, channels;
+    int64_t samples, positions, groups, cg, channels;
     int64_t run;        // samples a team takes
     Affine affine;
-    void *by_channel;   // C [row blocks * samples_at_once][2][channels], or null
+    void *by_channel;   // C [row blocks * samples_at_once * positions][2][channels], or null
 };
 
 // One launch; the group of a sample fits a team (t.v > 0). dispatch.
 hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation, const RowsForwardArgs &a);
-// positions == 1
 hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation, const RowsBackwardArgs &a, int64_t row_blocks);
 
-// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (4 and 16 without
-// vectors, 2 at least for a block).
+// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (4, 8 and 16
+// without vectors, 2 at least for a block).
 template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(const Teams &t, F &&f) {
     constexpr int V = kVector<T>, kMost = most_vectors(V, BACKWARD);
     const auto with = [&](auto v, auto k, auto wide) { return f(v, k, wide); };
@@ -213,6 +222,7 @@ template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(cons
     if (t.v == 1) {
         if (t.wide) return with(One{}, std::integral_constant<int, 16>{}, std::true_type{});
         if (t.k <= 4) return with(One{}, std::integral_constant<int, 4>{}, std::false_type{});
+        if (t.k <= 8) return with(One{}, std::integral_constant<int, 8>{}, std::false_type{});
         return with(One{}, std::integral_constant<int, 16>{}, std::false_type{});
     }
     if (t.wide) {

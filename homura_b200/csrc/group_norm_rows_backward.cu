@@ -1,5 +1,5 @@
-// Group norm with an activation, one position a sample and a group in the registers of a team of lanes: the gradients in
-// one pass; the split is group_norm_rows.cuh's. A team takes `run` samples one after another and keeps its channels' sums
+// Group norm with an activation where a group of one sample fits the registers of a team of lanes: the gradients in one
+// pass; the split is group_norm_rows.cuh's. A team takes `run` samples one after another and keeps its channels' sums
 // for dweight and dbias in registers (f32 for at most 64 samples, then a partial that is folded in f64).
 #include "group_norm_rows.cuh"
 
@@ -8,7 +8,7 @@ namespace gnorm {
 namespace {
 
 template <class T, int V, int K, bool WIDE, int ACT>
-__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_kernel(const __grid_constant__ RowsBackwardArgs a) {
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || K == 16 ? 1 : 2) rows_backward_kernel(const __grid_constant__ RowsBackwardArgs a) {
     using C = typename Comp<T>::C;
     constexpr bool kKeep = K * V <= 8;  // parameters in registers
     __shared__ C scratch[2][kWarps];
@@ -20,16 +20,20 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
     const int64_t group = static_cast<int64_t>(blockIdx.x) * a.t.groups_per_tile + (team - beside * a.t.groups_per_tile);
     const bool team_live = beside < a.t.samples_at_once && group < a.groups;
     const int64_t first_channel = group * a.cg;
-    const int at = lane * V, apart = a.t.lanes * V;  // this lane's first vector, and how far apart its vectors are
+    // this lane's vectors: position, first channel within the group
+    int position[K], at[K];
     bool have[K];
     C w[kKeep ? K : 1][V], b[kKeep ? K : 1][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        have[k] = team_live && lane + k * a.t.lanes < a.t.vectors;
+        const int vector = lane + k * a.t.lanes;
+        have[k] = team_live && vector < a.t.vectors;
+        position[k] = vector / a.t.row_vectors;
+        at[k] = (vector - position[k] * a.t.row_vectors) * V;
         if constexpr (kKeep) {
             if (have[k]) {
-                parameters<T, V>(w[k], a.affine.weight, first_channel + at + k * apart, a.affine.weight_stride, a.affine.is_f32, C(1));
-                parameters<T, V>(b[k], a.affine.bias, first_channel + at + k * apart, a.affine.bias_stride, a.affine.is_f32, C(0));
+                parameters<T, V>(w[k], a.affine.weight, first_channel + at[k], a.affine.weight_stride, a.affine.is_f32, C(1));
+                parameters<T, V>(b[k], a.affine.bias, first_channel + at[k], a.affine.bias_stride, a.affine.is_f32, C(0));
             }
         }
 #pragma unroll
@@ -38,17 +42,17 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
     const C share = C(1) / (static_cast<C>(a.t.vectors) * C(V));
     const int64_t first = static_cast<int64_t>(blockIdx.y) * a.run * a.t.samples_at_once;
     int64_t n = first + beside;
-    const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n + first_channel + at;
-    const T *dout = reinterpret_cast<const T *>(a.dout) + n * a.wdout.n + first_channel + at;
-    T *dsrc = reinterpret_cast<T *>(a.dsrc) + n * a.wdsrc.n + first_channel + at;
+    const T *src = reinterpret_cast<const T *>(a.src) + n * a.wsrc.n + first_channel;
+    const T *dout = reinterpret_cast<const T *>(a.dout) + n * a.wdout.n + first_channel;
+    T *dsrc = reinterpret_cast<T *>(a.dsrc) + n * a.wdsrc.n + first_channel;
     const int64_t src_next = a.t.samples_at_once * a.wsrc.n, dout_next = a.t.samples_at_once * a.wdout.n, dsrc_next = a.t.samples_at_once * a.wdsrc.n;
     const auto load = [&](int64_t sample, int64_t r, int stage) {
         if (r < a.run && sample < a.samples) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (have[k]) {
-                    ring.fetch(stage, k, src + k * apart);
-                    ring.fetch(stage, K + k, dout + k * apart);
+                    ring.fetch(stage, k, src + position[k] * a.wsrc.s + at[k]);
+                    ring.fetch(stage, K + k, dout + position[k] * a.wdout.s + at[k]);
                 }
             }
         }
@@ -83,8 +87,8 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
         for (int k = 0; k < K; ++k) {
             if constexpr (!kKeep) {
                 if (have[k]) {
-                    parameters<T, V>(w[0], a.affine.weight, first_channel + at + k * apart, a.affine.weight_stride, a.affine.is_f32, C(1));
-                    parameters<T, V>(b[0], a.affine.bias, first_channel + at + k * apart, a.affine.bias_stride, a.affine.is_f32, C(0));
+                    parameters<T, V>(w[0], a.affine.weight, first_channel + at[k], a.affine.weight_stride, a.affine.is_f32, C(1));
+                    parameters<T, V>(b[0], a.affine.bias, first_channel + at[k], a.affine.bias_stride, a.affine.is_f32, C(0));
                 }
             }
             if (!live || !have[k]) continue;
@@ -110,19 +114,20 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 ? 1 : 2) rows_backward_
             C y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) y[i] = rstd * (p[k][i] - m1 - xhat[k][i] * m2);
-            *reinterpret_cast<Pack<T, V> *>(dsrc + k * apart) = pack_of<T, V>(y);
+            *reinterpret_cast<Pack<T, V> *>(dsrc + position[k] * a.wdsrc.s + at[k]) = pack_of<T, V>(y);
         }
         dsrc += dsrc_next;
     }
     if (a.by_channel == nullptr || !team_live) return;
-    C *to = reinterpret_cast<C *>(a.by_channel) + (static_cast<int64_t>(blockIdx.y) * a.t.samples_at_once + beside) * 2 * a.channels + first_channel;
+    const int64_t partial = (static_cast<int64_t>(blockIdx.y) * a.t.samples_at_once + beside) * a.positions;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if (!have[k]) continue;
+        C *to = reinterpret_cast<C *>(a.by_channel) + (partial + position[k]) * 2 * a.channels + first_channel + at[k];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            to[(lane + k * a.t.lanes) * V + i] = dw[k][i];
-            to[a.channels + (lane + k * a.t.lanes) * V + i] = db[k][i];
+            to[i] = dw[k][i];
+            to[a.channels + i] = db[k][i];
         }
     }
 }

@@ -85,7 +85,7 @@ def test_recurrence_backward_refusals():
 def test_group_norm_refusals():
     lib = homura_b200.load()
     t, stat, par = desc([2, 3, 8]), desc([2, 4]), desc([8])
-    long = desc([2, 100000, 8])  # a group that no block holds: its pieces' moments need a workspace
+    long = desc([2, 3000000, 8])  # a group that no cluster holds: its pieces' moments need a workspace
     nbytes = ctypes.c_int64(-1)
     assert lib.hmc_group_norm_workspace(t, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value >= 0
     assert lib.hmc_group_norm_workspace(long, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value > 0
@@ -126,7 +126,7 @@ def test_group_norm_refusals():
     assert lib.hmc_group_norm_workspace(None, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     assert lib.hmc_group_norm_workspace(t, 5, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     # sizes alone decide: a description without memory is enough
-    assert lib.hmc_group_norm_workspace(desc([2, 100000, 8], data=False), 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value == need
+    assert lib.hmc_group_norm_workspace(desc([2, 3000000, 8], data=False), 4, 0, ctypes.byref(nbytes)) == ffi.HMC_OK and nbytes.value == need
 
 
 def test_group_norm_backward_refusals():
