@@ -230,6 +230,8 @@ inline hmc_status check_problem(const hmc_tensor_desc *src, int32_t groups, Prob
     int64_t n = 0;
     s = count_layer(src->sizes, 3, &n);
     if (s != HMC_OK) return s;
+    // (workspaces hold at most some tens of bytes an element: their sizes stay within 63 bits)
+    if (n > (int64_t{1} << 56)) return fail(HMC_INVALID, "the tensor has too many elements");
     const int64_t stats[2] = {src->sizes[0], groups};
     s = count_layer(stats, 2, &n);
     if (s != HMC_OK) return s;

@@ -32,8 +32,9 @@ extern "C" {
  * and may be the view `initial`) are [batch, channels] of F32 (F64 when T is F64). out may be the view x or the view
  * gate. The state is held in the computation type. A step with a = 0 forgets what came before it, whatever it was
  * unless that is infinite or NaN. With no time steps `last` receives `initial`. One step (time = 1) is the form for
- * generating a token. Gates may exceed 1 in magnitude as long as products of up to 4096 neighbouring gates stay in the
- * computation type's range. */
+ * generating a token. The time axis is folded in pieces of up to 128 steps: gates may exceed 1 in magnitude as long as
+ * products of that many neighbours stay in the computation type's range, and what an infinite state becomes where such a
+ * product underflows or a gate is infinite is NaN or an infinity. */
 hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_desc *out, const hmc_tensor_desc *gate,
                                  const hmc_tensor_desc *x, const hmc_tensor_desc *initial, const hmc_tensor_desc *last,
                                  int32_t flags);
@@ -59,8 +60,7 @@ hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_tensor_de
  * the view src. weight and bias (both or neither) are [channels] of T or of F32, alike. mean and rstd (both or neither)
  * receive the groups' moments, [samples, groups] of F32 (F64 when T is F64), for the backward pass. The moments are
  * taken in two passes over values held on chip (first the mean, then the deviations from it) and merged pairwise where
- * a group is cut into pieces. A NaN or an infinity makes its own group NaN (an infinity: every element of the group but
- * those of the activation's limits), no other. The workspace has hmc_group_norm_workspace bytes (0: NULL is fine),
+ * a group is cut into pieces. A NaN or an infinity makes its own group NaN, no other. The workspace has hmc_group_norm_workspace bytes (0: NULL is fine),
  * 16-byte aligned. */
 hmc_status hmc_group_norm_workspace(const hmc_tensor_desc *src, int32_t groups, int32_t backward, int64_t *bytes);
 hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out, const hmc_tensor_desc *src,

@@ -166,8 +166,9 @@ def activation(kind, z):
 def activation_error(kind, z, dtype):
     """Absolute error of the kernel's act(z) and act'(z) at an exact z: a few units of 1 + |z| (the exponential's argument
     carries its own rounding: |z| units, |z|^2 for gelu's density, whose factor e^(-z^2/2) keeps the product below one unit
-    each; gelu_tanh's inner polynomial carries 4 units of up to |z| (1 + z^2), beyond |z| = 5 times a vanishing slope); half
-    types through ex2.approx and rcp.approx, four times that."""
+    each; gelu_tanh's inner polynomial carries 4 units of up to |z| (1 + z^2), beyond |z| = 5 times a vanishing slope); f32 goes through ex2.approx
+    (2 units), rcp.approx (1) and, for gelu, a fit of erfc good to 1.2e-7 (2 units), which 16 hold; half types four times
+    that, for none of it is seen after their rounding."""
     if kind in (None, "none", "relu"):
         return np.zeros_like(z), np.zeros_like(z)
     u = unit(dtype) * (4 if dtype in (F16, BF16) else 1)

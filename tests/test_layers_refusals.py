@@ -123,6 +123,7 @@ def test_group_norm_refusals():
     refused(call(out=empty, src=empty, ws=None, n=0), "null context")
     refused(call(out=empty, src=empty, mean=stat, rstd=stat), "moments of empty groups")
     assert lib.hmc_group_norm_workspace(t, 4, 0, None) == ffi.HMC_INVALID
+    refused(lib.hmc_group_norm_workspace(desc([2**30, 2**20, 2**10], strides=[0, 0, 1]), 4, 0, ctypes.byref(nbytes)), "too many elements")
     assert lib.hmc_group_norm_workspace(None, 4, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     assert lib.hmc_group_norm_workspace(t, 5, 0, ctypes.byref(nbytes)) == ffi.HMC_INVALID
     # sizes alone decide: a description without memory is enough
