@@ -227,7 +227,7 @@ Plan make_plan(const Problem &p, Align align) {
 int64_t forward_workspace(const Problem &p) {
     const int es = element_size(p.dtype), vector = 16 / es;
     const auto need = [&](Align align) -> int64_t {
-        if (make_teams(p, vector, align == Align::kLine, false).v > 0 || find_resident(p, align, 1).t.v > 0) return 0;
+        if (make_teams(p, align, false).v > 0 || find_resident(p, align, 1).t.v > 0) return 0;
         return make_plan(p, align).bytes;
     };
     int64_t most = es >= 4 ? 0 : need(Align::kAny);
@@ -267,7 +267,7 @@ HMC_API hmc_status hmc_group_norm(hmc_context_t ctx, const hmc_tensor_desc *out,
         if (s != HMC_OK) return s;
         HMC_ENTER(ctx);
         const Align align = alignment(p.dtype, src, out);
-        const Teams teams = make_teams(p, 16 / element_size(p.dtype), align == Align::kLine, false);
+        const Teams teams = make_teams(p, align, false);
         if (teams.v > 0) {
             RowsForwardArgs r{};
             r.out = layer_base(out);

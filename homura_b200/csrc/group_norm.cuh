@@ -111,6 +111,11 @@ template <class C> struct alignas(2 * sizeof(C)) Two {
     C a, b;
 };
 
+template <int BYTES> __device__ __forceinline__ void copy_async(void *shared_dst, const void *src) {
+    if constexpr (BYTES == 16) async_copy_16(shared_dst, src);
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared_dst))), "l"(src), "n"(BYTES) : "memory");
+}
+
 // ---- tiles ----
 
 struct Tiling {

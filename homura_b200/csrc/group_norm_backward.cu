@@ -249,13 +249,13 @@ struct RowRuns {
     Teams t;
     int64_t run, row_blocks, partials, bytes;
 };
-RowRuns make_runs(const Problem &p, int vector, bool vectors) {
+RowRuns make_runs(const Problem &p, Align align) {
     RowRuns r{};
-    r.t = make_teams(p, vector, vectors, true);
+    r.t = make_teams(p, align, true);
     if (r.t.v == 0) return r;
     const int64_t rounds = ceil_div(p.samples, r.t.samples_at_once);
     int64_t run = ceil_div(rounds * r.t.tiles, 148 * 8);
-    run = run < 4 ? 4 : (run > 64 ? 64 : run);
+    run = run < 8 ? 8 : (run > 64 ? 64 : run);
     if (ceil_div(rounds, run) > 65535 || r.t.tiles > (int64_t{1} << 30)) {  // beyond a grid's second dimension
         r.t.v = 0;
         return r;
@@ -281,7 +281,7 @@ int64_t resident_columns(const Problem &p, const Resident &r) {
 int64_t backward_workspace(const Problem &p) {
     const int es = element_size(p.dtype), vector = 16 / es;
     const auto need = [&](Align align) -> int64_t {
-        const RowRuns r = make_runs(p, vector, align == Align::kLine);
+        const RowRuns r = make_runs(p, align);
         if (r.t.v > 0) return r.bytes;
         const Resident resident = find_resident(p, align, 2);
         if (resident.t.v > 0) {
@@ -371,7 +371,7 @@ HMC_API hmc_status hmc_group_norm_backward(hmc_context_t ctx, const hmc_tensor_d
             });
         }
         const Align align = alignment(p.dtype, src, dout, dsrc);
-        const RowRuns rows = make_runs(p, 16 / element_size(p.dtype), align == Align::kLine);
+        const RowRuns rows = make_runs(p, align);
         const Resident resident = rows.t.v > 0 ? Resident{} : find_resident(p, align, 2);
         const Plan plan = rows.t.v > 0 || resident.t.v > 0 ? Plan{} : make_plan(p, align);
         a.src = layer_base(src);

@@ -126,11 +126,6 @@ template <class C, int V> __device__ __forceinline__ Memory carve(unsigned char 
     return m;
 }
 
-template <int BYTES> __device__ __forceinline__ void copy_async(void *shared_dst, const void *src) {
-    if constexpr (BYTES == 16) async_copy_16(shared_dst, src);
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(shared_dst))), "l"(src), "n"(BYTES) : "memory");
-}
-
 // A thread's place in the columns for its V channels: of channel i at[i], in group[i] of the tile.
 template <int V> struct Columns {
     int at[V], group[V];

@@ -7,7 +7,7 @@ namespace gnorm {
 namespace {
 
 template <class T, int V, int K, bool WIDE, int ACT>
-__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || K == 16 ? 1 : (V > 1 && K * V <= 8 ? 3 : 2)) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
+__global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || (sizeof(T) * V == 2 && K == 16) ? 1 : (sizeof(T) * V == 16 && K * V <= 8 ? 3 : 2)) rows_kernel(const __grid_constant__ RowsForwardArgs a) {
     using C = typename Comp<T>::C;
     constexpr int U = samples_at_a_time(K);
     constexpr bool kKeep = K * V <= 16;  // parameters in registers
@@ -139,9 +139,10 @@ hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation,
             constexpr int V = decltype(v)::value, K = decltype(k)::value;
             constexpr bool WIDE = decltype(wide)::value;
             return dispatch_activation(activation, [&](auto act) -> hmc_status {
-                // about sixteen blocks an SM, each taking several rounds of samples with its parameters in registers
+                // blocks for some rounds each, so that the parameters and the first copies are paid once for many samples; more
+                // and shorter ones where two vectors a lane leave three blocks on an SM
                 const int64_t rounds = ceil_div(a.samples, static_cast<int64_t>(a.t.samples_at_once) * samples_at_a_time(K));
-                const int64_t wanted = ceil_div(148 * 16, a.t.tiles);
+                const int64_t wanted = ceil_div(148 * (K * V * static_cast<int>(sizeof(T)) <= 32 ? 16 : 4), a.t.tiles);
                 const int64_t y = rounds < wanted ? rounds : wanted;
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(y < 65535 ? y : 65535));
                 constexpr int kShared = RowRing<T, V, samples_at_a_time(K) * K>::kBytes;

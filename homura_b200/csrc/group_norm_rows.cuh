@@ -4,8 +4,8 @@
 // A team is a power of two of lanes within a warp (or, WIDE, the whole block); a lane keeps K vectors of V neighbouring
 // channels of its team's group, the same channels for every sample it takes, so parameters (and, backward, the sums for
 // dweight and dbias) stay in registers across samples. The next samples' vectors come through a ring in shared
-// memory that a lane's own asynchronous copies of 16 bytes fill rounds ahead (a lane reads only what it copied: waiting for
-// its copies is all the synchronisation); values without vectors are loaded to registers a round ahead. Sums go through shuffles within the team.
+// memory that a lane's own asynchronous copies fill rounds ahead (a lane reads only what it copied: waiting for its copies is
+// all the synchronisation). Sums go through shuffles within the team.
 #pragma once
 
 #include "group_norm.cuh"
@@ -13,8 +13,12 @@
 namespace hmc {
 namespace gnorm {
 
-// A lane's vectors at most: 32 values forward, 16 backward, where the sums for dweight and dbias stand beside them.
-constexpr int most_vectors(int v, bool backward) { return v == 1 ? 16 : ((backward ? 16 : 32) / v < 8 ? (backward ? 16 : 32) / v : 8); }
+// A lane's vectors at most: 32 values forward, 16 backward, where the sums for dweight and dbias stand beside them, in at
+// most eight vectors of 16 bytes or sixteen words (es: bytes of an element).
+constexpr int most_vectors(int v, int es, bool backward) {
+    const int most = (backward ? 16 : 32) / v, narrow = v * es < 16 ? 16 : 8;
+    return most < narrow ? most : narrow;
+}
 
 struct Teams {
     int32_t lanes;            // lanes a team
@@ -28,20 +32,28 @@ struct Teams {
     bool wide;
 };
 
-// The widest team that wastes least: K * lanes as small as possible, lanes as many as possible for coalescing.
-inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backward) {
+// K as it is compiled (dispatch_vectors).
+constexpr int compiled_k(int k, int v, int es, bool backward) {
+    const int most = most_vectors(v, es, backward);
+    int c = v * es == 16 ? 1 : 4;
+    while (c < k) c *= 2;
+    return c < most ? c : most;
+}
+// The widest team that wastes least: lanes * compiled K as small as possible, lanes as many as possible for coalescing.
+inline Teams make_teams(const Problem &p, Align align, bool backward) {
     Teams t{};
     const int64_t cg = p.channels / p.groups;
-    const int v = vectors && cg % vector == 0 ? vector : 1;
-    const int most_k = most_vectors(v, backward);
+    const int es = element_size(p.dtype), vector = 16 / es, word = narrow_vector(es);
+    const int v = align == Align::kLine && cg % vector == 0 ? vector : (align != Align::kAny && cg % word == 0 ? word : 1);
+    const int most_k = most_vectors(v, es, backward);
     const int64_t most = static_cast<int64_t>(kBlock) * most_k;
     if (p.positions > most || cg / v > most || p.positions * (cg / v) > most) return t;
     t.v = v;
     t.vectors = static_cast<int32_t>(p.positions * (cg / v));
     t.row_vectors = static_cast<int32_t>(cg / v);
-    // Single values of several rows are read in small pieces, at some 150 GB/s; a cluster reads them side by side but spends
+    // Words of several rows are read in small pieces, at some 150 GB/s; a cluster reads them side by side but spends
     // about 4 us a sample on two blocks an SM, which only samples of about 2 KB (all operands) do not repay.
-    if (v == 1 && p.positions > 1 && p.positions * p.channels * element_size(p.dtype) * (backward ? 3 : 2) > 2048) {
+    if (v < vector && p.positions > 1 && p.positions * p.channels * es * (backward ? 3 : 2) > 2048) {
         t.v = 0;
         return t;
     }
@@ -58,8 +70,9 @@ inline Teams make_teams(const Problem &p, int vector, bool vectors, bool backwar
         for (int lanes = 32; lanes >= 1; lanes >>= 1) {
             const int k = (t.vectors + lanes - 1) / lanes;
             if (k > most_k) break;
-            if (best == 0 || lanes * k < best) {
-                best = lanes * k;
+            const int cost = lanes * compiled_k(k, v, es, backward);
+            if (best == 0 || cost < best) {
+                best = cost;
                 t.lanes = lanes;
                 t.k = k;
             }
@@ -143,22 +156,20 @@ template <class T, int V> __device__ __forceinline__ Pack<T, V> pack_of(const ty
     return r;
 }
 
-// `WORDS` vectors a lane and round.
+// `WORDS` vectors (of 4, 8 or 16 bytes) a lane and round; single values of 2 bytes, for which there is no asynchronous copy,
+// are loaded to registers a round ahead.
 template <class T, int V, int WORDS> struct RowRing {
-    static constexpr bool kUsed = static_cast<int>(sizeof(T)) * V == 16;
-    static constexpr int kRound = WORDS * kBlock * 16;  // bytes a block and round
+    static constexpr int kSize = static_cast<int>(sizeof(T)) * V;
+    static constexpr bool kUsed = kSize >= 4;
+    static constexpr int kRound = WORDS * kBlock * kSize;  // bytes a block and round
     static constexpr int kStages = !kUsed ? 1 : (kRound * 4 <= 49152 ? 4 : (kRound * 3 <= 49152 ? 3 : 2));
     static constexpr int kBytes = kUsed ? kStages * kRound : 0;
     Pack<T, V> direct[kUsed ? 1 : WORDS];
     unsigned char *mine;
-    __device__ __forceinline__ explicit RowRing(unsigned char *memory) : mine(memory + threadIdx.x * 16) {}
+    __device__ __forceinline__ explicit RowRing(unsigned char *memory) : mine(memory + threadIdx.x * kSize) {}
     __device__ __forceinline__ void fetch(int stage, int word, const T *p) {
-        if constexpr (kUsed) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine + (stage * WORDS + word) * (kBlock * 16)))), "l"(p)
-                         : "memory");
-        } else {
-            direct[word] = *reinterpret_cast<const Pack<T, V> *>(p);
-        }
+        if constexpr (kUsed) copy_async<kSize>(mine + (stage * WORDS + word) * (kBlock * kSize), p);
+        else direct[word] = *reinterpret_cast<const Pack<T, V> *>(p);
     }
     // After the copies of a round; then, before the first read of the oldest round in flight.
     __device__ __forceinline__ void commit() const {
@@ -168,7 +179,7 @@ template <class T, int V, int WORDS> struct RowRing {
         if constexpr (kUsed) asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
     }
     __device__ __forceinline__ Pack<T, V> get(int stage, int word) const {
-        if constexpr (kUsed) return *reinterpret_cast<const Pack<T, V> *>(mine + (stage * WORDS + word) * (kBlock * 16));
+        if constexpr (kUsed) return *reinterpret_cast<const Pack<T, V> *>(mine + (stage * WORDS + word) * (kBlock * kSize));
         else return direct[word];
     }
 };
@@ -212,29 +223,36 @@ struct RowsBackwardArgs {
 hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation, const RowsForwardArgs &a);
 hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation, const RowsBackwardArgs &a, int64_t row_blocks);
 
-// f(V, K, WIDE) as compile-time constants: K is the next of 1, 2, 4 and 8 (4, 8 and 16
-// without vectors, 2 at least for a block).
-template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(const Teams &t, F &&f) {
-    constexpr int V = kVector<T>, kMost = most_vectors(V, BACKWARD);
-    const auto with = [&](auto v, auto k, auto wide) { return f(v, k, wide); };
-    using One = std::integral_constant<int, 1>;
-    using Vec = std::integral_constant<int, V>;
-    if (t.v == 1) {
-        if (t.wide) return with(One{}, std::integral_constant<int, 16>{}, std::true_type{});
-        if (t.k <= 4) return with(One{}, std::integral_constant<int, 4>{}, std::false_type{});
-        if (t.k <= 8) return with(One{}, std::integral_constant<int, 8>{}, std::false_type{});
-        return with(One{}, std::integral_constant<int, 16>{}, std::false_type{});
-    }
+// f(V, K, WIDE) as compile-time constants. K is the next of 1, 2, 4 and 8, of 4, 8 and 16 for words and single values; 2 at
+// least, or the most, for a block.
+template <class T, bool BACKWARD, int V, class F> inline hmc_status dispatch_vectors(const Teams &t, F &&f) {
+    constexpr int kMost = most_vectors(V, sizeof(T), BACKWARD);
+    constexpr bool kLines = V * sizeof(T) == 16;
+    const auto with = [&](auto k, auto wide) { return f(std::integral_constant<int, V>{}, k, wide); };
     if (t.wide) {
-        if (t.k <= 2) return with(Vec{}, std::integral_constant<int, 2>{}, std::true_type{});
-        return with(Vec{}, std::integral_constant<int, kMost>{}, std::true_type{});
+        if constexpr (kLines) {
+            if (t.k <= 2) return with(std::integral_constant<int, 2>{}, std::true_type{});
+        }
+        return with(std::integral_constant<int, kMost>{}, std::true_type{});
     }
-    if (t.k <= 1) return with(Vec{}, One{}, std::false_type{});
-    if (t.k <= 2) return with(Vec{}, std::integral_constant<int, 2>{}, std::false_type{});
-    if constexpr (kMost >= 4) {
-        if (t.k <= 4) return with(Vec{}, std::integral_constant<int, 4>{}, std::false_type{});
+    if constexpr (kLines) {
+        if (t.k <= 1) return with(std::integral_constant<int, 1>{}, std::false_type{});
+        if (t.k <= 2) return with(std::integral_constant<int, 2>{}, std::false_type{});
     }
-    return with(Vec{}, std::integral_constant<int, kMost>{}, std::false_type{});
+    if constexpr (kMost > 4) {
+        if (t.k <= 4) return with(std::integral_constant<int, 4>{}, std::false_type{});
+    }
+    if constexpr (kMost > 8) {
+        if (t.k <= 8) return with(std::integral_constant<int, 8>{}, std::false_type{});
+    }
+    return with(std::integral_constant<int, kMost>{}, std::false_type{});
+}
+template <class T, bool BACKWARD, class F> inline hmc_status dispatch_teams(const Teams &t, F &&f) {
+    if (t.v == kVector<T>) return dispatch_vectors<T, BACKWARD, kVector<T>>(t, f);
+    if constexpr (sizeof(T) == 2) {
+        if (t.v == 2) return dispatch_vectors<T, BACKWARD, 2>(t, f);
+    }
+    return dispatch_vectors<T, BACKWARD, 1>(t, f);
 }
 
 }  // namespace gnorm
