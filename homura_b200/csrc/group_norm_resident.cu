@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
 hmc_status launch_resident_forward(hmc_context_t ctx, int dtype, int32_t activation, const ResidentForwardArgs &a) {
     return dispatch_float(dtype, [&](auto tag) -> hmc_status {
         using T = decltype(tag);
-        return dispatch_activation(activation, [&](auto act) -> hmc_status {
+        if constexpr (std::is_same_v<T, double>) return fail(HMC_INTERNAL_ERROR, "F64 moments are merged from pieces");  // (make_resident)
+        else return dispatch_activation(activation, [&](auto act) -> hmc_status {
             const int64_t units = a.samples * a.r.t.tiles;
             const int64_t most = (int64_t{1} << 30) / a.r.cluster;
             if (a.r.t.v == kVector<T>) {

@@ -231,7 +231,8 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
             if (time == 1) return launch_forward<T, V, 1, 0>(ctx, a, batch, flags);
             const bool flat = flat_columns(channels, V), lines = wide && !flat;
             if constexpr (sizeof(T) < 8) {
-                // Sixteen rows a lane halve the exchanges, two blocks an SM then: where that many blocks take all channels.
+                // Sixteen rows a lane halve the exchanges, two blocks an SM then: where that many blocks take all channels (bf16
+                // [8, 2048, 4096]: 112 us with eight rows and four blocks an SM, 85 with sixteen).
                 const int64_t warps = flat ? ceil_div(batch * channels, int64_t{32} * V) : batch * ceil_div(channels, int64_t{32} * V);
                 if (warps <= int64_t{148} * 2 * kWarps) {
                     return lines ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);

@@ -6,12 +6,15 @@
  * homura has none of them (its layers are compositions of the operators of homura_cuda.h), so nothing here replaces a
  * declaration of csrc/homura_rocm.h; the rules of homura_cuda.h hold: status and message, the context's stream, the
  * thread's device restored, nothing queued by a failing call, workspaces from the caller, results that repeat bit for
- * bit (every sum is folded in an order fixed by the sizes). Arguments are checked before the context is looked at.
+ * bit (every sum is folded in an order fixed by sizes, dtypes and alignment). Arguments are checked before the context is
+ * looked at.
  *
  * The descriptions here are not merged: they have exactly the dimensions named below, in that order, sizes of 1
  * included. Strides are any non-negative numbers of elements (an input may broadcast by a stride of 0, the elements of
  * an output are distinct) unless an entry says more. T is F16, BF16, F32 or F64; the computation type is f32, for F64
- * f64; each result is rounded to its dtype once. Optional descriptions are NULL when absent.
+ * f64; each result is rounded to its dtype once. Optional descriptions are NULL when absent. A workspace is in use until
+ * the call's kernels have run: a later call on the same context may take it again, calls that may run at the same time
+ * (on two contexts, in two graphs) need one each.
  */
 #ifndef HOMURA_CUDA_LAYERS_H
 #define HOMURA_CUDA_LAYERS_H
