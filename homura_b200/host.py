@@ -975,27 +975,28 @@ class AdamWGroup:
         return out
 
 
-def plain_desc(kernel: str, t: Optional[TensorData]) -> Optional[hmc_tensor_desc]:
-    """The description of a tensor dimension by dimension, none merged or dropped; None stays None."""
-    if t is None:
-        return None
-    n = len(t.shape)
-    if n > MAX_DIMS:
-        raise BackendError(ffi.HMC_INVALID, f"{kernel} on CUDA supports at most {MAX_DIMS} dimensions, got {n}")
-    if CHECK_REACH:
-        check_reach(kernel, t, t.offset, [(size, [st]) for size, st in zip(t.shape, t.strides)], 0)
-    return packed_desc(t, t.shape, t.strides)
-
-
 # A description packed in one go: a third of the time of setting its fields one by one, of which a small kernel's call has
 # as many as it has operands.
 _PACK_DESC = [struct.Struct(f"<Qqii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x") for n in range(MAX_DIMS + 1)]
 assert all(s.size == ctypes.sizeof(hmc_tensor_desc) for s in _PACK_DESC)
+_PACK_DESC = [s.pack for s in _PACK_DESC]
+_desc_from = hmc_tensor_desc.from_buffer_copy
 
 
 def packed_desc(t: TensorData, shape: Sequence[int], strides: Sequence[int]) -> hmc_tensor_desc:
-    n = len(shape)
-    return hmc_tensor_desc.from_buffer_copy(_PACK_DESC[n].pack(t.storage.address, t.offset, t.dtype, n, *shape, *strides))
+    n, storage = len(shape), t.storage
+    return _desc_from(_PACK_DESC[n](storage.ptr if storage.array is None else storage.address, t.offset, t.dtype, n, *shape, *strides))
+
+
+def plain_desc(kernel: str, t: Optional[TensorData]) -> Optional[hmc_tensor_desc]:
+    """The description of a tensor dimension by dimension, none merged or dropped; None stays None."""
+    if t is None:
+        return None
+    if len(t.shape) > MAX_DIMS:
+        raise BackendError(ffi.HMC_INVALID, f"{kernel} on CUDA supports at most {MAX_DIMS} dimensions, got {len(t.shape)}")
+    if CHECK_REACH:
+        check_reach(kernel, t, t.offset, [(size, [st]) for size, st in zip(t.shape, t.strides)], 0)
+    return packed_desc(t, t.shape, t.strides)
 
 
 def channels_last_desc(kernel: str, t: TensorData) -> hmc_tensor_desc:
