@@ -896,15 +896,16 @@ class CudaBackend:
         self._dropout("dropout_backward", dsrc, dout, None, p, state)
 
     def _dropout(self, kernel: str, out: TensorData, src: TensorData, residual: Optional[TensorData], p: float, state: tuple) -> None:
-        operands = [out, src] if residual is None else [out, src, residual]
-        if out.numel == 0 or any(t.shape != out.shape for t in operands):
+        operands = (out, src) if residual is None else (out, src, residual)
+        shape, strides, n = out.shape, out.strides, out.numel
+        alike = src.shape == shape and (residual is None or residual.shape == shape)
+        if n == 0 or not alike:
             d = [plain_desc(kernel, t) for t in operands]  # nothing to write, or refused by the library
-        elif all(t.is_contiguous() for t in operands):
-            n, step = (out.numel,), (1,)
+        elif src.strides == strides and (residual is None or residual.strides == strides) and out.is_contiguous():
             if CHECK_REACH:
                 for t in operands:
-                    check_reach(kernel, t, t.offset, [(n[0], [1])], 0)
-            d = [packed_desc(t, n, step) for t in operands]
+                    check_reach(kernel, t, t.offset, [(n, [1])], 0)
+            d = [packed_desc(t, (n,), (1,)) for t in operands]
         else:
             d = descs(kernel, operands)
         self._check(self.lib.hmc_dropout(self.ctx, d[0], d[1], d[2] if len(d) > 2 else None, float(p), *state))
