@@ -242,3 +242,14 @@ def test_two_backends_at_once(cuda):
             assert (be.download(out) == want).all()
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("dtype,size", [(F32, (1, 60000, 64, 2)), (BF16, (1, 9000, 532, 2)), (F16, (2, 9001, 531, 1)), (F32, (1, 30001, 33, 1)),
+                                        (BF16, (3, 20000, 256, 1))],
+                         ids=["f32 lines", "bf16 words", "f16 odd", "f32 words", "bf16 lines"])
+def test_groups_beyond_a_cluster(cuda, dtype, size):
+    """Groups whose rows no cluster's shared memory holds: pieces that a second kernel merges."""
+    rng = np.random.default_rng(sum(size))
+    check_forward(cuda, rng, size, dtype, "silu", True)
+    check_backward(cuda, rng, size, dtype, "silu", True)
+    check_backward(cuda, rng, size, dtype, "relu", False, F32 if dtype != F32 else None)
