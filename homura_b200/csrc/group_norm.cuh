@@ -56,7 +56,9 @@ template <class C> __device__ __forceinline__ C gelu_inner(C z, C &slope) {
 }
 
 // xhat * w + b: in two roundings before relu, whose derivative goes by the sign alone, so that the sign is that of the
-// plain formula; fused otherwise. Forward and backward take the same steps.
+// plain formula; fused otherwise. Every forward and backward kernel takes the same steps from x on, (x - mean) * rstd first,
+// so that all find the same z: moments and parameters are not folded into one product and sum, which leaves
+// mean * rstd * 2^-24 of noise (0.4 for a group of 30000s, whose z is its bias).
 template <int ACT, class C> __device__ __forceinline__ C scaled(C xhat, C w, C b) {
     if constexpr (ACT == HMC_UNARY_RELU) return xhat * w + b;
     else return m_fma(xhat, w, b);

@@ -129,16 +129,6 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
             }
             parameters<T, V>(w, a.affine.weight, channel, a.affine.weight_stride, a.affine.is_f32, C(1));
             parameters<T, V>(b, a.affine.bias, channel, a.affine.bias_stride, a.affine.is_f32, C(0));
-            // For 2-byte elements moments and parameters fold into one product and sum: what that rounds (2^-24 of mean * rstd)
-            // is far below the step of an element that is that far from the others.
-            constexpr bool kFolded = sizeof(T) == 2;
-            if constexpr (kFolded) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    w[i] *= rstd[i];
-                    b[i] = m_fma(-mean[i], w[i], b[i]);
-                }
-            }
             T *out = reinterpret_cast<T *>(a.out) + sample * a.wout.n + (first + ty) * a.wout.s + channel;
             const int64_t step = t.ty * a.wout.s;
 #pragma unroll 2
@@ -146,10 +136,7 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
                 const Pack<T, V> x = mine[k * kBlock];
                 C y[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if constexpr (kFolded) y[i] = activate<ACT>(m_fma(up(x.v[i]), w[i], b[i]));
-                    else y[i] = activate<ACT>(scaled<ACT>((up(x.v[i]) - mean[i]) * rstd[i], w[i], b[i]));
-                }
+                for (int i = 0; i < V; ++i) y[i] = activate<ACT>(scaled<ACT>((up(x.v[i]) - mean[i]) * rstd[i], w[i], b[i]));
                 *reinterpret_cast<Pack<T, V> *>(out) = pack_of<T, V>(y);
             }
         }

@@ -1,0 +1,48 @@
+"""Where the trainable operators of include/homura_cuda_layers.h could go wrong by more than rounding: groups of one value, signs
+at an activation's kink, long sums, logits and values at the ends of their types. Expected values are exact or follow from
+the definition; a tolerance counts the roundings on a value's way."""
+import numpy as np
+import pytest
+
+from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS
+from layers_reference import raw, value
+
+pytestmark = pytest.mark.gpu
+
+stat_dtype = lambda dtype: F64 if dtype == F64 else F32
+
+
+def norm(be, x, dtype, groups, weight=None, bias=None, kind=None, eps=1e-5):
+    """Forward with F32 (F64) parameters: out, mean and rstd as stored."""
+    out = be.empty(x.shape, dtype)
+    stats = [be.empty((x.shape[0], groups), stat_dtype(dtype)) for _ in range(2)]
+    up = lambda v: None if v is None else be.upload(raw(v, stat_dtype(dtype)), stat_dtype(dtype))
+    be.group_norm(out, be.upload(x, dtype), groups, up(weight), up(bias), *stats, eps=eps, activation=kind)
+    return be.download(out), be.download(stats[0]), be.download(stats[1])
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=[DTYPE_NAMES[d] for d in FLOATS])
+@pytest.mark.parametrize("size", [(1, 512, 4), (200, 64, 4), (77, 320, 32), (390, 58, 2), (33, 257, 1), (60000, 64, 2)], ids=str)
+def test_relu_passes_gradients_exactly_where_it_passed_values(cuda, dtype, size):
+    """The bias puts the value in the middle of each channel on relu's kink: forward and backward have to take it for the same
+    side. With a gradient of 1 everywhere dbias counts the elements that the backward pass took for positive."""
+    s, c, groups = size
+    rng = np.random.default_rng(sum(size))
+    sd = stat_dtype(dtype)
+    real = np.float64 if dtype == F64 else np.float32
+    # some hundred above a spread of a few: steps of the half types are 1 and 1/4 there
+    x = raw((192 + rng.integers(-8, 9, (1, s, c))).astype(np.float64), dtype)
+    _, mean, rstd = norm(cuda, x, dtype, groups)
+    wide = lambda v: np.repeat(v, c // groups, 1)[0]
+    w = rng.uniform(0.5, 2, c).astype(real)
+    middle = value(x, dtype)[0, s // 2].astype(real)
+    b = -((middle - wide(mean)) * wide(rstd) * w)
+    out, mean2, rstd2 = norm(cuda, x, dtype, groups, w, b, "relu")
+    assert (mean == mean2).all() and (rstd == rstd2).all()
+    out = value(out, dtype)[0]
+    assert (out[s // 2] == 0).all()
+    up = lambda v: cuda.upload(np.ascontiguousarray(v), sd)
+    dx, dw, db = cuda.empty(x.shape, dtype), cuda.empty((c,), sd), cuda.empty((c,), sd)
+    cuda.group_norm_backward(dx, cuda.upload(x, dtype), cuda.upload(raw(np.ones(x.shape), dtype), dtype), up(mean), up(rstd), groups,
+                             up(w), up(b), dw, db, activation="relu")
+    assert (cuda.download(db) == (out > 0).sum(0)).all(), np.abs(cuda.download(db) - (out > 0).sum(0)).max()
