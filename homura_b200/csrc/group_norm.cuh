@@ -91,6 +91,14 @@ template <int ACT, class C> __device__ __forceinline__ C through(C d, C z) {
 __device__ __forceinline__ float inverse_root(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
 
+// sum / count from share = 1 / count rounded: the product with share is off by up to an ulp and a half where count is no
+// power of two, and one step of Newton's method on it gives every quotient that the type holds, so that the mean of a constant
+// group is its value. What is no finite number keeps the product.
+template <class C> __device__ __forceinline__ C quotient(C sum, C count, C share) {
+    const C q = sum * share, rest = m_fma(-q, count, sum);
+    return rest == rest ? m_fma(rest, share, q) : q;
+}
+
 // ---- operands ----
 
 // weight and bias, or null; of T or of f32.

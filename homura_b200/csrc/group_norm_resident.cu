@@ -65,9 +65,9 @@ __global__ void __launch_bounds__(kBlock, 2) resident_kernel(const __grid_consta
                 }
             }
             if (have > 0) {
-                const C share = C(1) / static_cast<C>(have);
+                const C rows_here = static_cast<C>(have), share = C(1) / rows_here;
 #pragma unroll
-                for (int i = 0; i < V; ++i) mean[i] = many ? static_cast<C>(total[i] / have) : sum[i] * share;
+                for (int i = 0; i < V; ++i) mean[i] = many ? static_cast<C>(total[i] / have) : quotient(sum[i], rows_here, share);
             }
             if (many) {
 #pragma unroll

@@ -21,6 +21,30 @@ def norm(be, x, dtype, groups, weight=None, bias=None, kind=None, eps=1e-5):
     return be.download(out), be.download(stats[0]), be.download(stats[1])
 
 
+# rows in registers, a cluster's shared memory (with and without whole vectors) and pieces; groups whose size is a power of two
+# and groups whose reciprocal size is not a number of the computation type
+CONSTANT = [(3, 1, 64, 4), (3, 1, 60, 6), (3, 1, 4998, 3), (2, 200, 64, 4), (2, 77, 320, 32), (2, 390, 58, 2), (1, 3000, 16, 1), (2, 33, 257, 1),
+            (1, 60000, 64, 2)]
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=[DTYPE_NAMES[d] for d in FLOATS])
+@pytest.mark.parametrize("size", CONSTANT, ids=str)
+def test_a_constant_group_becomes_its_bias(cuda, dtype, size):
+    """Sums of these values and their quotient by the size are exact, so the mean is the value, every deviation is 0 and the
+    output the bias, whatever the weight."""
+    n, s, c, groups = size
+    rng = np.random.default_rng(sum(size))
+    w, b = rng.normal(1, 0.3, c), rng.normal(0, 0.3, c)
+    for level in (0.0, 3.25, -1000.0, 30000.0):
+        x = raw(np.full((n, s, c), level), dtype)
+        got, mean, rstd = norm(cuda, x, dtype, groups, w, b)
+        want = raw(np.broadcast_to(raw(b, stat_dtype(dtype)).astype(np.float64), x.shape), dtype)
+        assert (mean == value(x, dtype)[0, 0, 0]).all(), (level, mean)
+        # 1 / sqrt(eps), eps rounded to the computation type, by a function good to two units in the last place
+        assert (np.abs(rstd * np.sqrt(1e-5) - 1) <= (4 * 2.0**-52 if dtype == F64 else 4 * 2.0**-23)).all(), (level, rstd)
+        assert (value(got, dtype) == value(want, dtype)).all(), (level, np.abs(value(got, dtype) - value(want, dtype)).max())
+
+
 @pytest.mark.parametrize("dtype", FLOATS, ids=[DTYPE_NAMES[d] for d in FLOATS])
 @pytest.mark.parametrize("size", [(1, 512, 4), (200, 64, 4), (77, 320, 32), (390, 58, 2), (33, 257, 1), (60000, 64, 2)], ids=str)
 def test_relu_passes_gradients_exactly_where_it_passed_values(cuda, dtype, size):
