@@ -1,8 +1,8 @@
 // Group norm with an activation, channels last, the gradients (include/homura_cuda_layers.h); tiles as in group_norm.cuh.
 //
 // Three steps: sums over each run of rows of dz and dz * xhat (by channel for weight and bias, by group, weighted, for
-// the input), a small kernel that folds the runs in order, and an elementwise pass. Channel sums are kept in f64 across
-// the runs a block takes, and folded over the blocks in f64.
+// the input), a small kernel that folds the runs in order, and an elementwise pass. A thread adds at most 64 rows of a
+// run in the computation type. Channel sums are kept in f64 across the runs a block takes, and folded over the blocks in f64.
 #include <algorithm>
 
 #include "group_norm_resident.cuh"
@@ -233,6 +233,13 @@ Plan make_plan(const Problem &p, Align align) {
     // (a tiling by lines that does not come out is one by single values; by words it may)
     if (align == Align::kLine && r.t.v == 1) r.t = make_tiling(p.channels, p.groups, narrow_vector(es), true);
     r.sums = cut_rows(p, r.t, static_cast<int64_t>(r.t.ty) * 4);
+    // however many strips there are, a thread adds no more than 64 rows in the computation type
+    const int64_t most = static_cast<int64_t>(r.t.ty) * 64;
+    if (r.sums.run > most) {
+        r.sums.run = most;
+        r.sums.chunks = ceil_div(p.positions, most);
+        r.sums.units = p.samples * r.t.tiles * r.sums.chunks;
+    }
     r.apply = cut_rows(p, r.t, r.t.ty);
     const int64_t pairs = p.samples * r.sums.chunks;
     r.columns = ceil_div(kBlocksWanted, r.t.tiles);

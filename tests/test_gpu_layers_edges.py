@@ -70,3 +70,24 @@ def test_relu_passes_gradients_exactly_where_it_passed_values(cuda, dtype, size)
     cuda.group_norm_backward(dx, cuda.upload(x, dtype), cuda.upload(raw(np.ones(x.shape), dtype), dtype), up(mean), up(rstd), groups,
                              up(w), up(b), dw, db, activation="relu")
     assert (cuda.download(db) == (out > 0).sum(0)).all(), np.abs(cuda.download(db) - (out > 0).sum(0)).max()
+
+
+def one_large_many_small(be, large, s, c, n, dtype, groups):
+    """dbias and dweight where dout is 2048 in the rows `large` and 2^-13 in all others, half a unit of f32 at 2048, so that an f32
+    sum that has 2048 in it loses every addition; x = 1, mean = 0, rstd = 1. Samples are one sample, by a stride of 0."""
+    d = np.full((1, s, c), 2.0**-13)
+    d[0, large] = 2048.0
+    src = be.upload(raw(np.ones((1, s, c)), dtype), dtype).expand(n, s, c)
+    dout = be.upload(raw(d, dtype), dtype).expand(n, s, c)
+    stat = lambda v: be.upload(np.full((1, groups), v, np.float32), F32).expand(n, groups)
+    dx, dw, db = be.empty((n, s, c), dtype), be.empty((c,), F32), be.empty((c,), F32)
+    be.group_norm_backward(dx, src, dout, stat(0), stat(1), groups, None, None, dw, db)
+    return be.download(dw), be.download(db), n * d[0, :, 0].sum()
+
+
+def test_sums_over_long_runs_of_rows(cuda):
+    """As many strips as blocks, so a run is every position, one row at a time: at most 64 are added in f32, then in f64."""
+    dw, db, want = one_large_many_small(cuda, [0], 2000, 129, 600, F16, 1)
+    for got in (dw, db):
+        # 64 roundings of the f32 sum, one of the product with the weight, half a step of the result
+        assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
