@@ -861,6 +861,7 @@ class CudaBackend:
         ([samples, groups], F32, or F64 for F64 tensors) receive for the backward pass. `activation`: None, "relu", "silu",
         "gelu" or "gelu_tanh". `weight` and `bias` ([channels]) have src's dtype or F32. `out` may be the view `src`."""
         k = "group_norm"
+        check_positions(k, src, out)
         s = channels_last_desc(k, src)
         ws, ptr, nbytes = self._group_norm_workspace(s, groups, 0)
         self._check(self.lib.hmc_group_norm(self.ctx, channels_last_desc(k, out), s, plain_desc(k, weight), plain_desc(k, bias),
@@ -874,6 +875,7 @@ class CudaBackend:
         """The gradients of :meth:`group_norm` into `dsrc` and (unless None) `dweight` and `dbias`, from its operands, the
         moments it left and the gradient `dout`. `dsrc` may be the view `dout` or `src`."""
         k = "group_norm_backward"
+        check_positions(k, src, dsrc, dout)
         s = channels_last_desc(k, src)
         ws, ptr, nbytes = self._group_norm_workspace(s, groups, 1)
         self._check(self.lib.hmc_group_norm_backward(
@@ -1017,6 +1019,16 @@ def channels_last_desc(kernel: str, t: TensorData) -> hmc_tensor_desc:
                                             f"{tuple(t.strides)} are not evenly spaced")
     size, (stride,) = between[0]
     return plain_desc(kernel, TensorData(t.storage, t.dtype, (t.shape[0], size, t.shape[-1]), (t.strides[0], stride, t.strides[-1]), t.offset))
+
+
+def check_positions(kernel: str, src: TensorData, *others: TensorData) -> None:
+    """Operands of one number of positions may still disagree about their rows and columns ([2, 4, 6, 8] and [2, 6, 4, 8]). One may
+    have the positions of another in one dimension."""
+    between = [n for n in src.shape[1:-1] if n != 1]
+    for t in others:
+        theirs = [n for n in t.shape[1:-1] if n != 1]
+        if len(theirs) == len(between) and theirs != between:
+            raise BackendError(ffi.HMC_INVALID, f"{kernel}: operands of shapes {tuple(src.shape)} and {tuple(t.shape)}")
 
 
 def recurrence_flags(sigmoid: bool, complement: bool, reverse: bool) -> int:

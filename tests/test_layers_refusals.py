@@ -7,8 +7,8 @@ import pytest
 
 import homura_b200
 from homura_b200 import ffi
-from homura_b200.host import (BF16, F16, F32, F64, I32, ACTIVATIONS, BackendError, Storage, TensorData, activation_code,
-                              channels_last_desc, contiguous_strides, plain_desc, recurrence_flags)
+from homura_b200.host import (BF16, F16, F32, F64, I32, ACTIVATIONS, BackendError, CudaBackend, Storage, TensorData, activation_code,
+                              channels_last_desc, check_positions, contiguous_strides, plain_desc, recurrence_flags)
 
 HOST = np.zeros(1 << 16, dtype=np.uint8)  # an address that is not null; no call here gets as far as using it
 
@@ -206,3 +206,19 @@ def test_every_declared_symbol_of_the_layers_is_exported():
                      "hmc_linear_recurrence", "hmc_linear_recurrence_backward"]
     for n in names:
         assert hasattr(homura_b200.load(), n) and n in ffi.FUNCTIONS
+
+
+def test_positions_in_another_order_are_refused():
+    """[2, 4, 6, 8] and [2, 6, 4, 8] both have 24 positions; they are not the same ones. The positions in one dimension, or with
+    dimensions of 1 between them, are."""
+    fake = lambda *shape: TensorData(Storage(16, array=HOST), F32, shape, contiguous_strides(shape))
+    maps, turned = fake(2, 4, 6, 8), fake(2, 6, 4, 8)
+    be, stats = object.__new__(CudaBackend), fake(2, 4)  # (refused before the backend is looked at)
+    with pytest.raises(BackendError, match="shapes"):
+        be.group_norm(turned, maps, 4)
+    with pytest.raises(BackendError, match="shapes"):
+        be.group_norm_backward(turned, maps, maps, stats, stats, 4)
+    with pytest.raises(BackendError, match="shapes"):
+        be.group_norm_backward(maps, maps, turned, stats, stats, 4)
+    check_positions("group_norm", maps, maps, fake(2, 24, 8), fake(2, 4, 1, 6, 8))
+    check_positions("group_norm", fake(2, 8), fake(2, 1, 8))
