@@ -56,18 +56,45 @@ __global__ void __launch_bounds__(kBlock, 2) resident_backward_kernel(const __gr
             rstd[i] = live ? reinterpret_cast<const C *>(a.rstd)[sample * a.rstd_n + group * a.rstd_g] : C(0);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // (vectors of 8 and 16 bytes: shared memory holds at most 54 and 27 rows of a thread; words up to 108, whose sums go on in
+        // f64 every 64 rows)
+        constexpr int kRun = 64;
         C s1[V], s2[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) s1[i] = s2[i] = C(0);
+        const auto add = [&](int k0, int k1) {
 #pragma unroll 2
-        for (int k = 0; k < have; ++k) {
-            const Pack<T, V> x = xs[k * kBlock], d = ds[k * kBlock];
+            for (int k = k0; k < k1; ++k) {
+                const Pack<T, V> x = xs[k * kBlock], d = ds[k * kBlock];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const C xhat = (up(x.v[i]) - mean[i]) * rstd[i];
-                const C dz = through<ACT>(up(d.v[i]), scaled<ACT>(xhat, w[i], b[i]));
-                s1[i] += dz;
-                s2[i] = m_fma(dz, xhat, s2[i]);
+                for (int i = 0; i < V; ++i) {
+                    const C xhat = (up(x.v[i]) - mean[i]) * rstd[i];
+                    const C dz = through<ACT>(up(d.v[i]), scaled<ACT>(xhat, w[i], b[i]));
+                    s1[i] += dz;
+                    s2[i] = m_fma(dz, xhat, s2[i]);
+                }
+            }
+        };
+        if constexpr (kResidentShared / (2 * kBlock * kBytes) <= kRun) {
+            add(0, have);
+        } else {
+            double t1[V], t2[V];
+            for (int k0 = 0; k0 < have; k0 += kRun) {
+                add(k0, k0 + kRun < have ? k0 + kRun : have);
+                if (have <= kRun) break;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    t1[i] = static_cast<double>(s1[i]) + (k0 > 0 ? t1[i] : 0.0);
+                    t2[i] = static_cast<double>(s2[i]) + (k0 > 0 ? t2[i] : 0.0);
+                    s1[i] = s2[i] = C(0);
+                }
+            }
+            if (have > kRun) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s1[i] = static_cast<C>(t1[i]);
+                    s2[i] = static_cast<C>(t2[i]);
+                }
             }
         }
         if (live) {

@@ -91,3 +91,11 @@ def test_sums_over_long_runs_of_rows(cuda):
     for got in (dw, db):
         # 64 roundings of the f32 sum, one of the product with the weight, half a step of the result
         assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
+
+
+def test_sums_over_a_clusters_rows(cuda):
+    """Words in a cluster's shared memory, 98 rows a thread, the first of each thread large."""
+    rows = [r for r in range(6272) if r % 784 < 8]
+    dw, db, want = one_large_many_small(cuda, rows, 6272, 58, 1, F16, 2)
+    for got in (dw, db):
+        assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
