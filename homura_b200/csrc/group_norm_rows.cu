@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || (sizeof(T) * V == 2 
         }
     }
     const C count = static_cast<C>(a.t.vectors) * C(V), share = C(1) / count;
+    const bool exact = (a.t.vectors & (a.t.vectors - 1)) == 0;  // then share is (V is a power of two)
     const int64_t step = static_cast<int64_t>(a.t.samples_at_once) * U * gridDim.y;
     const int64_t first = static_cast<int64_t>(blockIdx.y) * a.t.samples_at_once * U;
     int64_t n = first + beside;  // of the samples at a time, samples_at_once apart, the first
@@ -93,7 +94,7 @@ __global__ void __launch_bounds__(kBlock, sizeof(T) == 8 || (sizeof(T) * V == 2 
         team_sum<U, WIDE>(mean, a.t.lanes, scratch);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            mean[u] = quotient(mean[u], count, share);
+            mean[u] = exact ? mean[u] * share : quotient(mean[u], count, share);
             sq[u] = C(0);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
