@@ -81,9 +81,11 @@ template <int ACT, class C> __device__ __forceinline__ C through(C d, C z) {
     } else if constexpr (ACT == HMC_UNARY_GELU) {
         return d * m_fma(z, density(z), normal_cdf(z));
     } else if constexpr (ACT == HMC_UNARY_GELU_TANH) {
+        // (beyond 64 s is 0 or 1 to the last bit, but the inner slope and its product with z overflow in the end: held there)
         C slope;
-        const C s = logistic(gelu_inner(z, slope));
-        return d * (s * m_fma(z * (C(1) - s), slope, C(1)));
+        const C s = logistic(gelu_inner(z, slope)), held = z > C(64) ? C(64) : (z < C(-64) ? C(-64) : z);
+        gelu_inner(held, slope);
+        return d * (s * m_fma(held * (C(1) - s), slope, C(1)));
     } else return d;
 }
 

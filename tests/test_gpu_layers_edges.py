@@ -99,3 +99,25 @@ def test_sums_over_a_clusters_rows(cuda):
     dw, db, want = one_large_many_small(cuda, rows, 6272, 58, 1, F16, 2)
     for got in (dw, db):
         assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32, F64], ids=["bf16", "f32", "f64"])
+@pytest.mark.parametrize("size", [(2, 1, 64, 2), (2, 90, 64, 4), (1, 33, 257, 1)], ids=str)
+def test_gradients_far_out_on_an_activation(cuda, dtype, size):
+    """Where an activation's slope is 0 or 1 to the last bit the gradient is 0 or dout, however large the value, in the types that
+    hold such values; mean = 0 and rstd = 1, so the activation sees the input."""
+    n, s, c, groups = size
+    rng = np.random.default_rng(sum(size))
+    sd = stat_dtype(dtype)
+    up = lambda v, dt: cuda.upload(raw(v, dt), dt)
+    for far in (200.0, 1e10, 1e14, 1e18, 1e20, 3e38) + ((1e60, 1e120, 1e300) if dtype == F64 else ()):
+        sign = rng.integers(0, 2, (n, s, c)) * 2.0 - 1
+        d = value(raw(rng.normal(size=(n, s, c)), dtype), dtype)
+        for kind in ("relu", "silu", "gelu", "gelu_tanh"):
+            dx, db = cuda.empty((n, s, c), dtype), cuda.empty((c,), sd)
+            cuda.group_norm_backward(dx, up(sign * far, dtype), up(d, dtype), up(np.zeros((n, groups)), sd), up(np.ones((n, groups)), sd),
+                                     groups, None, None, None, db, activation=kind)
+            got, want, size_of = cuda.download(db), np.where(sign > 0, d, 0.0).sum((0, 1)), np.abs(d).sum((0, 1))
+            # a slope of 1 within the 32 units of 1 + |z| at z = 200 of tests/layers_reference.py, at most n s additions
+            u = 2.0**-53 if dtype == F64 else 2.0**-24
+            assert (np.abs(got - want) <= (40 + n * s) * u * size_of).all(), (kind, far, got, want)
