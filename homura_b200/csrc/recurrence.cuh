@@ -107,15 +107,6 @@ template <class T, int V> __device__ __forceinline__ Vec<typename Comp<T>::C, V>
 template <class C, int V> struct Gates {
     Vec<C, V> a, rest;
 };
-// Logits of half types held at -87 or above, NaN passed on.
-__device__ __forceinline__ uint32_t at_least_87(uint32_t pair, F16) {
-    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(pair) : "r"(0xD570D570u));
-    return pair;
-}
-__device__ __forceinline__ uint32_t at_least_87(uint32_t pair, BF16) {
-    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(pair) : "r"(0xC2AEC2AEu));
-    return pair;
-}
 template <bool SIG, class T, int V> __device__ __forceinline__ Gates<typename Comp<T>::C, V> gates_of(Pack<T, V> stored) {
     using C = typename Comp<T>::C;
     Gates<C, V> r;
@@ -124,23 +115,19 @@ template <bool SIG, class T, int V> __device__ __forceinline__ Gates<typename Co
 #pragma unroll
         for (int i = 0; i < V; ++i) r.rest.v[i] = C(1) - r.a.v[i];
     } else if constexpr (sizeof(T) == 2) {
-        // rounded to at most 11 bits later. e = exp(-g) stays below 2^126, so that both approximations stay in range (a is
-        // e^-87 where it should be less)
-        if constexpr (V == 2) {
-            uint32_t pair;
-            memcpy(&pair, &stored, 4);
-            pair = at_least_87(pair, T{});
-            memcpy(&stored, &pair, 4);
-        }
-        Vec<C, V> t = widen<T, V>(stored), e;
-        if constexpr (V == 1) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t.v[0]) : "f"(-87.0f));
-        t = vmul(t, splat<C, V>(-1.44269504088896341f));
+        // The special function unit's exponential and reciprocal: a and 1 - a to (12 + 2 |g|) 2^-24, for logits of 8 or 11 bits.
+        // Where e = exp(-g) passes 2^126 the reciprocal is flushed to 0, so that a logit of -infinity forgets whatever it meets, and
+        // e a is 0 or no number: 1 - a, less what its terms may be off by, is below e a everywhere else and stands in for it there.
+        const Vec<C, V> g = widen<T, V>(stored), t = vmul(g, splat<C, V>(-1.44269504088896341f));
+        Vec<C, V> e;
 #pragma unroll
         for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v[i]) : "f"(t.v[i]));
-        t = vadd(e, splat<C, V>(1.0f));
+        const Vec<C, V> all = vadd(e, splat<C, V>(1.0f));
 #pragma unroll
-        for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.a.v[i]) : "f"(t.v[i]));
-        r.rest = vmul(e, r.a);
+        for (int i = 0; i < V; ++i) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.a.v[i]) : "f"(all.v[i]));
+        const Vec<C, V> product = vmul(e, r.a), low = vfma(r.a, splat<C, V>(-1.0f), splat<C, V>(1.0f - 0x1p-21f));
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.rest.v[i] = fmaxf(product.v[i], low.v[i]);  // (no number only for a NaN logit)
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {

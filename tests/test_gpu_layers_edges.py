@@ -121,3 +121,35 @@ def test_gradients_far_out_on_an_activation(cuda, dtype, size):
             # a slope of 1 within the 32 units of 1 + |z| at z = 200 of tests/layers_reference.py, at most n s additions
             u = 2.0**-53 if dtype == F64 else 2.0**-24
             assert (np.abs(got - want) <= (40 + n * s) * u * size_of).all(), (kind, far, got, want)
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=[DTYPE_NAMES[d] for d in FLOATS])
+@pytest.mark.parametrize("channels", [64, 7, 300])
+def test_a_logit_of_minus_infinity_forgets(cuda, dtype, channels):
+    """sigmoid(-inf) is 0: nothing of the state before is left, however large that is, in the outputs, the state and the
+    gradients."""
+    rng = np.random.default_rng(channels)
+    sd = stat_dtype(dtype)
+    large = 60000.0 if dtype == F16 else 1e37
+    for t in (1, 2, 9, 300):
+        gate, x = rng.normal(size=(2, t, channels)), rng.normal(size=(2, t, channels))
+        k = t // 2
+        gate[:, k] = -np.inf
+        x[:, k] = 0.0
+        x[:, :k] = large
+        gate[:, :k] = -20.0
+        up = lambda v: cuda.upload(raw(v, dtype), dtype)
+        out, last = cuda.empty((2, t, channels), dtype), cuda.empty((2, channels), sd)
+        first = cuda.upload(raw(np.full((2, channels), large), sd), sd)
+        cuda.linear_recurrence(out, up(gate), up(x), first, last, sigmoid=True)
+        got = value(cuda.download(out), dtype)
+        assert (got[:, k] == 0).all(), np.abs(got[:, k]).max()
+        if k == t - 1:
+            assert (cuda.download(last) == 0).all()
+        # dinitial is the product of all gates, dgate has the factor a
+        dgate, dx, di = cuda.empty((2, t, channels), dtype), cuda.empty((2, t, channels), dtype), cuda.empty((2, channels), sd)
+        dlast = cuda.upload(raw(np.full((2, channels), 0.1), sd), sd)
+        cuda.linear_recurrence_backward(dgate, dx, up(gate), None, out, up(np.full((2, t, channels), 0.1)), first, dlast, di, sigmoid=True)
+        if k == 0:
+            assert (cuda.download(di) == 0).all()
+        assert (value(cuda.download(dgate), dtype)[:, k] == 0).all()
