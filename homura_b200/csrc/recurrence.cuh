@@ -37,12 +37,9 @@ template <class C> struct alignas(2 * sizeof(C)) Step {
     C a, b;
 };
 
-// A step applied to the value before it.
-template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return m_fma(s.a, v, s.b); }
-// A product of gates that has overflowed is held at the largest finite number, so that a state of zero before it stays
-// zero instead of becoming NaN. (A NaN or infinite gate shows in b already, which is folded from zero.)
-__device__ __forceinline__ float finite(float a) { return fminf(fmaxf(a, -3.4028234663852886e38f), 3.4028234663852886e38f); }
-__device__ __forceinline__ double finite(double a) { return fmin(fmax(a, -1.7976931348623157e308), 1.7976931348623157e308); }
+// A step applied to the value before it. A product of gates may have overflowed: a state of zero stays zero all the same, any
+// other becomes infinite or no number, never a finite wrong one. (A NaN or infinite gate shows in b, which is folded from zero.)
+template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return v == C(0) ? s.b : m_fma(s.a, v, s.b); }
 
 // Rows and channels of one operand, in elements; t may be negative.
 struct Walk {
@@ -432,7 +429,7 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
     {
         Pair mine_packed;
 #pragma unroll
-        for (int i = 0; i < V; ++i) mine_packed.v[i] = Step<C>{finite(a.v[i]), b.v[i]};
+        for (int i = 0; i < V; ++i) mine_packed.v[i] = Step<C>{a.v[i], b.v[i]};
         *reinterpret_cast<Pair *>(&warps[first + p.wt][p.slot]) = mine_packed;
     }
     __syncthreads();
@@ -455,8 +452,6 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
                     t.v[i].a *= s.v[i].a;
                 }
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i) t.v[i].a = finite(t.v[i].a);
             send<C, V>(&x.block[generation][p.rank][p.slot], &x.arrived[generation], p.wt, t);
         }
         await(&x.arrived[generation], (round >> 1) & 1u, status, gave_up);

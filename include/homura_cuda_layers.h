@@ -37,8 +37,10 @@ extern "C" {
  * gate. The state is held in the computation type. A step with a = 0 forgets what came before it, whatever it was
  * unless that is infinite or NaN. With no time steps `last` receives `initial`. One step (time = 1) is the form for
  * generating a token. The time axis is folded in pieces of up to 128 steps: gates may exceed 1 in magnitude as long as
- * products of that many neighbours stay in the computation type's range, and what an infinite state becomes where such a
- * product underflows or a gate is infinite is NaN or an infinity. */
+ * products of that many neighbours stay in the computation type's range. Where one overflows, a state of zero before the piece
+ * still gives the right results, any other an infinity or NaN; where one underflows, less than the type's smallest number
+ * times the state is lost. What an infinite state becomes where a product underflows or a gate is infinite is NaN or an
+ * infinity. */
 hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_desc *out, const hmc_tensor_desc *gate,
                                  const hmc_tensor_desc *x, const hmc_tensor_desc *initial, const hmc_tensor_desc *last,
                                  int32_t flags);

@@ -153,3 +153,28 @@ def test_a_logit_of_minus_infinity_forgets(cuda, dtype, channels):
         if k == 0:
             assert (cuda.download(di) == 0).all()
         assert (value(cuda.download(dgate), dtype)[:, k] == 0).all()
+
+
+def test_products_of_gates_beyond_the_range_show(cuda):
+    """Gates whose product leaves f32 within a piece, with states that stay in it (the header asks for gates whose products stay
+    in range): a result is right or no finite number, never a finite wrong one, and a state of zero stays zero."""
+    for t in (60, 300, 5000):
+        apart, within_a_lane = np.full(t, 0.5), np.full(t, 0.5)
+        apart[:50] = 30.0        # 1e-38 becomes 7e35, the product of 50 gates is 7e73, those of 16 are in range
+        apart[50] = 0.0          # and infinity times 0 would be no number where the reset leaves x
+        within_a_lane[:8] = 1e6  # 1e-38 becomes 1e10, the product of 8 gates is 1e48
+        for gates in (apart, within_a_lane):
+            for start in (0.0, 1e-38):
+                x = np.zeros(t)
+                x[50] = 1.0
+                want, h = np.zeros(t), start
+                for k in range(t):
+                    h = gates[k] * h + x[k]
+                    want[k] = h
+                row = lambda v: cuda.upload(v.astype(np.float32), F32)
+                out = cuda.empty((1, t, 33), F32)
+                cuda.linear_recurrence(out, row(gates[None, :, None]).expand(1, t, 33), row(x[None, :, None]).expand(1, t, 33), row(np.full((1, 33), start)))
+                got = cuda.download(out)[0].astype(np.float64)
+                # three roundings a step, and as many again where a piece is folded first; subnormals are rounded absolutely
+                right = np.abs(got - want[:, None]) <= 6 * t * 2.0**-24 * np.abs(want[:, None]) + 2.0**-126
+                assert (right | ((start != 0.0) & ~np.isfinite(got))).all(), (t, start, got[~right][:4])
