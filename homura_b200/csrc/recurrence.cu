@@ -14,6 +14,7 @@ struct ForwardArgs {
     int64_t time, channels;
     Columns columns;
     int32_t warps_time;
+    int32_t wait_limit;
     int *status;
 };
 
@@ -35,7 +36,6 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
     const int64_t mine = static_cast<int64_t>(R) * (p.rank * a.warps_time + p.wt);
     begin_exchange(shared, p);
     uint32_t rounds = 0;
-    bool gave_up = false;
     for (int64_t item = blockIdx.x / p.cluster; item < a.columns.items; item += gridDim.x / p.cluster) {
         const Column at_column = column_of<V>(a.columns, item, a.warps_time, p.wc, p.lane);
         const int64_t batch = at_column.batch, channel = at_column.channel;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
                     sum = vfma(ca[r], sum, cu[r]);
                     product = vmul(product, ca[r]);
                 }
-                exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, h, carry, a.status, gave_up);
+                exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, h, carry, a.wait_limit, a.status);
             }
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, per_sm<T>(R)) forward_kernel(const _
             for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.last)[batch * a.wlast.b + (channel + i) * a.wlast.c] = carry.v[i];
         }
     }
-    end_exchange(p);
+    end_exchange(shared, p);
 }
 
 template <class T, int V, int R, int COPY>
@@ -182,7 +182,12 @@ hmc_status launch_forward(hmc_context_t ctx, ForwardArgs &a, int64_t batch, int3
     return dispatch_flags(flags, go);
 }
 
+thread_local int polls_of_a_wait = kPollLimit;
+
 }  // namespace
+
+int wait_limit() { return polls_of_a_wait; }
+
 }  // namespace recur
 }  // namespace hmc
 
@@ -219,6 +224,7 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
         a.wlast = walk_state(last);
         a.time = time;
         a.channels = channels;
+        a.wait_limit = wait_limit();
         a.status = ctx->status;
         const bool pairs = layer_vectors(out, 4) && layer_vectors(gate, 4) && layer_vectors(x, 4);
         const bool wide = layer_vectors(gate, 16) && layer_vectors(x, 16) && layer_vectors(out, 4);
@@ -242,3 +248,5 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
         });
     });
 }
+
+HMC_API void hmc_test_wait_limit(int32_t polls) { polls_of_a_wait = polls >= 0 ? polls : kPollLimit; }

@@ -359,6 +359,7 @@ template <class C, int V> struct alignas(16) Exchange {
     Step<C> block[2][kMaxCluster][32 * V];
     C carry[2][kWarps][32 * V];   // by the warp's place along channels
     alignas(8) uint64_t arrived[2];
+    int gave_up;                  // a thread of the block has given up a wait
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -369,12 +370,25 @@ template <class C, int V> __device__ __forceinline__ void begin_exchange(Exchang
     if (threadIdx.x == 0) {
         for (int g = 0; g < 2; ++g) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[g])) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        x.gave_up = 0;
     }
     cg::this_cluster().sync();  // every block runs, its barriers stand, before anyone writes to its shared memory
 }
-// After the last: no block ends while another may still write to it.
-__device__ __forceinline__ void end_exchange(const Place &p) {
-    if (p.cluster > 1) cg::this_cluster().sync();
+template <class C, int V> __device__ __forceinline__ bool has_given_up(const Exchange<C, V> &x) {
+    return *static_cast<const volatile int *>(&x.gave_up) != 0;
+}
+// After the last: no block ends while another may still write to it. A block that has seen every round's sums arrive knows of
+// nothing on its way; for one that gave up, what its neighbours had sent by the barrier gets far more time than the microsecond
+// that a store between blocks takes (2^14 looks, some 100 us).
+template <class C, int V> __device__ __forceinline__ void end_exchange(Exchange<C, V> &x, const Place &p) {
+    if (p.cluster == 1) return;
+    cg::this_cluster().sync();
+    if (!has_given_up(x)) return;
+#pragma unroll 1
+    for (int look = 0; look < 1 << 14; ++look) {
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%0], 0;\n\t}" ::"r"(shared_address(&x.arrived[look & 1]))
+                     : "memory");
+    }
 }
 
 // One lane's V steps to the same place of another block, counted off on that block's mbarrier.
@@ -395,13 +409,17 @@ template <class C, int V> __device__ __forceinline__ void send(const Step<C> *mi
 }
 
 constexpr int kPollLimit = 1 << 22;
+// Polls of a wait: kPollLimit, or what the calling thread has set for its tests (hmc_test_wait_limit).
+int wait_limit();
 
-// A wait that gives up: no block waits for ever for one that never sends. `status` is the context's word; once a thread has
-// given up it waits no more.
-__device__ __forceinline__ void await(uint64_t *arrived, uint32_t parity, int *status, bool &gave_up) {
-    if (gave_up) return;
-    const uint32_t at = shared_address(arrived);
-    for (int poll = 0; poll < kPollLimit; ++poll) {
+// A wait for the sums of a round that gives up after `limit` polls. `status` is the context's word. A block of which a thread has
+// given up waits no more and, from the next round on, sends no more and expects no more: a neighbour that misses its sums gives
+// up in turn, and nobody touches a barrier or sums of a round that its block has not seen complete. (The barriers of the whole
+// cluster at the kernel's begin and end are the hardware's, among blocks that run at the same time.)
+template <class C, int V> __device__ __forceinline__ void await(Exchange<C, V> &x, uint32_t generation, uint32_t parity, int limit, int *status) {
+    const uint32_t at = shared_address(&x.arrived[generation]);
+#pragma unroll 1
+    for (int poll = 0; poll < limit; ++poll) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -409,8 +427,9 @@ __device__ __forceinline__ void await(uint64_t *arrived, uint32_t parity, int *s
             : "r"(at), "r"(parity)
             : "memory");
         if (done) return;
+        if (has_given_up(x)) return;
     }
-    gave_up = true;
+    *static_cast<volatile int *>(&x.gave_up) = 1;
     atomicExch(status, 1);
 }
 
@@ -420,7 +439,7 @@ __device__ __forceinline__ void await(uint64_t *arrived, uint32_t parity, int *s
 // lane keeps.
 template <class C, int V>
 __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int warps_time, uint32_t round, bool first_round,
-                                         const Vec<C, V> &a, const Vec<C, V> &b, Vec<C, V> &v, Vec<C, V> &carry, int *status, bool &gave_up) {
+                                         const Vec<C, V> &a, const Vec<C, V> &b, Vec<C, V> &v, Vec<C, V> &carry, int limit, int *status) {
     using Pair = Pack<Step<C>, V>;
     const uint32_t generation = round & 1u;
     Step<C>(&warps)[kWarps][32 * V] = x.warp[generation];
@@ -434,14 +453,14 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
     }
     __syncthreads();
     if (p.cluster > 1) {
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && !has_given_up(x)) {
             asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&x.arrived[generation])),
                          "r"(static_cast<uint32_t>(p.cluster * 32 * V * sizeof(Step<C>)))
                          : "memory");
         }
         // (a cluster is used with all eight warps along time only, so a block has one tile of channels; warp w brings the
         // block's fold to block w)
-        if (p.wt < p.cluster) {
+        if (p.wt < p.cluster && !has_given_up(x)) {
             Pair t = at(warps[0]);
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) {
@@ -454,7 +473,7 @@ __device__ __forceinline__ void exchange(Exchange<C, V> &x, const Place &p, int 
             }
             send<C, V>(&x.block[generation][p.rank][p.slot], &x.arrived[generation], p.wt, t);
         }
-        await(&x.arrived[generation], (round >> 1) & 1u, status, gave_up);
+        await(x, generation, (round >> 1) & 1u, limit, status);
 #pragma unroll 4
         for (int k = 0; k < p.cluster; ++k) {
             const Pair s = at(x.block[generation][k]);

@@ -17,6 +17,7 @@ struct BackwardArgs {
     int64_t time, channels;
     Columns columns;
     int32_t warps_time;
+    int32_t wait_limit;
     int *status;
 };
 
@@ -39,7 +40,6 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
     const int64_t mine = static_cast<int64_t>(R) * (p.rank * a.warps_time + p.wt);
     begin_exchange(shared, p);
     uint32_t rounds = 0;
-    bool gave_up = false;
     for (int64_t item = blockIdx.x / p.cluster; item < a.columns.items; item += gridDim.x / p.cluster) {
         const Column at_column = column_of<V>(a.columns, item, a.warps_time, p.wc, p.lane);
         const int64_t batch = at_column.batch, channel = at_column.channel;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
             if (n == R) read(std::true_type{});
             else read(std::false_type{});
             Vec<C, V> g = carry;
-            if (!alone) exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, g, carry, a.status, gave_up);
+            if (!alone) exchange(shared, p, a.warps_time, rounds, base == 0, product, sum, g, carry, a.wait_limit, a.status);
             const auto write = [&](auto whole) {
                 constexpr bool kWhole = decltype(whole)::value;  // (and the last row in processing order is not among them)
                 T *to_gate = pdgate, *to_x = pdx;
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T>) backward_kernel(const __g
             for (int i = 0; i < V; ++i) reinterpret_cast<C *>(a.dinitial)[batch * a.wdinitial.b + (channel + i) * a.wdinitial.c] = carry.v[i];
         }
     }
-    end_exchange(p);
+    end_exchange(shared, p);
 }
 
 template <class T, int V, int R, int COPY>
@@ -264,6 +264,7 @@ HMC_API hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_t
         a.wdlast = walk_state(dlast);
         a.time = time;
         a.channels = channels;
+        a.wait_limit = wait_limit();
         a.status = ctx->status;
         const bool pairs = layer_vectors(dgate, 4) && layer_vectors(dx, 4) && layer_vectors(gate, 4) && layer_vectors(out, 4) &&
                            layer_vectors(dout, 4) && (!complement || layer_vectors(x, 4));

@@ -235,6 +235,7 @@ FUNCTIONS = {
     "hmc_test_reduce_plan": (c_int32, [(POINTER(hmc_tensor_desc), "kept"), (POINTER(hmc_tensor_desc), "red"), (POINTER(c_int64), "kind"), (POINTER(c_int64), "splits"), (POINTER(c_int64), "chunk")]),
     "hmc_test_softmax_plan": (c_int32, [(POINTER(hmc_tensor_desc), "src_rows"), (c_int64, "n"), (c_int64, "src_stride"), (POINTER(c_int32), "kind"), (POINTER(c_int32), "group"), (POINTER(c_int32), "cache")]),
     "hmc_test_index_value": (c_int32, [(c_void_p, "ctx"), (POINTER(hmc_tensor_desc), "index"), (POINTER(c_uint64), "slot")]),
+    "hmc_test_wait_limit": (None, [(c_int32, "polls")]),
     "hmc_test_live_streams": (c_int32, []),
     "hmc_test_current_device": (c_int32, [(POINTER(c_int32), "device")]),
     "hmc_test_set_current_device": (c_int32, [(c_int32, "device")]),

@@ -488,6 +488,8 @@ void hmc_abi_check(hmc_abi_info *out);
  *   reduce: kind (0 rows, 1 columns, 2 generic), splits of the reduced range, elements per split.
  *   softmax: kind (0 row in registers, 1 streaming, 2 row staged in shared memory by a warp, 3 few long
  *   rows split into three launches), lanes per row, vectors a lane keeps.
+ * wait_limit(n): the bounded waits of the thread's next calls of hmc_linear_recurrence(_backward) give up after n polls (n < 0: the
+ *   usual number); n = 0 makes every wait give up at once.
  * live_streams: streams the thread created and has not destroyed. */
 void hmc_test_fail_stream_create(int32_t n);
 void hmc_test_fail_after_probe(int32_t n);
@@ -501,6 +503,7 @@ hmc_status hmc_test_softmax_plan(const hmc_tensor_desc *src_rows, int64_t n, int
  * UINT64_MAX, writes the value there to slot[1]: to test positions far beyond what a check could reach in a test
  * (2^60 and more, in views with zero strides). `slot` is device memory. csrc/homura_rocm.h:631-634, 657-658 */
 hmc_status hmc_test_index_value(hmc_context_t ctx, const hmc_tensor_desc *index, uint64_t *slot);
+void hmc_test_wait_limit(int32_t polls);
 int32_t hmc_test_live_streams(void);
 hmc_status hmc_test_current_device(int32_t *device);
 hmc_status hmc_test_set_current_device(int32_t device);

@@ -4,7 +4,7 @@ the definition; a tolerance counts the roundings on a value's way."""
 import numpy as np
 import pytest
 
-from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS
+from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS, BackendError, CudaBackend
 from layers_reference import raw, value
 
 pytestmark = pytest.mark.gpu
@@ -178,3 +178,37 @@ def test_products_of_gates_beyond_the_range_show(cuda):
                 # three roundings a step, and as many again where a piece is folded first; subnormals are rounded absolutely
                 right = np.abs(got - want[:, None]) <= 6 * t * 2.0**-24 * np.abs(want[:, None]) + 2.0**-126
                 assert (right | ((start != 0.0) & ~np.isfinite(got))).all(), (t, start, got[~right][:4])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32, F64], ids=["bf16", "f32", "f64"])
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable(dtype):
+    """The blocks of a cluster wait for one another's sums with a limit. With a limit of 0 all give up at once, every peer alive: the
+    kernel ends, the next synchronisation says so once, and the following calls give the same bits as before."""
+    rng = np.random.default_rng(1)
+    be, sd = CudaBackend(0), stat_dtype(dtype)
+    try:
+        up = lambda v: be.upload(raw(v, dtype), dtype)
+        for t in (300, 5000):
+            gate, x, d = (up(rng.normal(size=(2, t, 34))) for _ in range(3))
+            out, last = be.empty((2, t, 34), dtype), be.empty((2, 34), sd)
+            dgate, dx, di = be.empty((2, t, 34), dtype), be.empty((2, t, 34), dtype), be.empty((2, 34), sd)
+            forward = lambda: be.linear_recurrence(out, gate, x, None, last, sigmoid=True)
+            backward = lambda: be.linear_recurrence_backward(dgate, dx, gate, None, out, d, None, None, di, sigmoid=True)
+            forward(), backward()
+            be.synchronize()
+            want = [be.download(v) for v in (out, last, dgate, dx, di)]
+            for call in (forward, backward):
+                be.lib.hmc_test_wait_limit(0)
+                try:
+                    call()
+                finally:
+                    be.lib.hmc_test_wait_limit(-1)
+                with pytest.raises(BackendError, match="gave up a bounded wait"):
+                    be.synchronize()
+                be.synchronize()
+            forward(), backward()
+            be.synchronize()
+            for a, v in zip(want, [be.download(v) for v in (out, last, dgate, dx, di)]):
+                assert (a == v).all()
+    finally:
+        be.close()
