@@ -888,8 +888,13 @@ class CudaBackend:
         """out = (residual +) src with every element dropped with probability p and the kept ones divided by 1 - p. The
         mask is a function of the returned (seed, first block) and of the element's row-major position: hand the pair to
         :meth:`dropout_backward`. `out` may be the view `src` or `residual`."""
-        state = gen.reserve(-(-src.numel // 4))
-        self._dropout("dropout", out, src, residual, p, state)
+        blocks = -(-src.numel // 4)
+        state = gen.reserve(blocks)
+        try:
+            self._dropout("dropout", out, src, residual, p, state)
+        except Exception:
+            gen.give_back(state, blocks)
+            raise
         return state
 
     def dropout_backward(self, dsrc: TensorData, dout: TensorData, p: float, state: tuple) -> None:
@@ -1121,6 +1126,11 @@ class Generator:
         start = self.offset
         self.offset = (self.offset + blocks) & (2**64 - 1)
         return self.seed, start
+
+    def give_back(self, state: tuple, blocks: int) -> None:
+        """The blocks of a call that was refused, unless others have been reserved behind them since."""
+        if (self.seed, self.offset) == (state[0], (state[1] + blocks) & (2**64 - 1)):
+            self.offset = state[1]
 
 
 def int_range(low: int, high: int) -> tuple[int, int]:

@@ -7,7 +7,7 @@ import pytest
 
 import homura_b200
 from homura_b200 import ffi
-from homura_b200.host import (BF16, F16, F32, F64, I32, ACTIVATIONS, BackendError, CudaBackend, Storage, TensorData, activation_code,
+from homura_b200.host import (BF16, F16, F32, F64, I32, ACTIVATIONS, BackendError, CudaBackend, Generator, Storage, TensorData, activation_code,
                               channels_last_desc, check_positions, contiguous_strides, plain_desc, recurrence_flags)
 
 HOST = np.zeros(1 << 16, dtype=np.uint8)  # an address that is not null; no call here gets as far as using it
@@ -222,3 +222,23 @@ def test_positions_in_another_order_are_refused():
         be.group_norm_backward(maps, maps, turned, stats, stats, 4)
     check_positions("group_norm", maps, maps, fake(2, 24, 8), fake(2, 4, 1, 6, 8))
     check_positions("group_norm", fake(2, 8), fake(2, 1, 8))
+
+
+def test_a_refused_dropout_leaves_the_generator_where_it_was():
+    """Nothing was drawn, so the next call's mask is the one it would have had."""
+    fake = lambda shape, dtype=F32: TensorData(Storage(16, array=HOST), dtype, shape, contiguous_strides(shape))
+    be = object.__new__(CudaBackend)  # (a context that is null: the library refuses every call)
+    be.lib, be.ctx = homura_b200.load(), None
+    gen = Generator(7)
+    gen.reserve(5)
+    for shape, p in (((3, 5), 0.5), ((3, 5), 2.0), ((0,), 0.5)):
+        with pytest.raises(BackendError):
+            be.dropout(fake(shape), fake(shape), gen, p)
+        assert gen.offset == 5
+    with pytest.raises(BackendError, match="wrong sizes"):
+        be.dropout(fake((4,)), fake((5,)), gen, 0.5)
+    assert gen.offset == 5
+    first = gen.reserve(3)
+    gen.reserve(1)
+    gen.give_back(first, 3)  # another call has drawn since: what it drew stays its own
+    assert gen.offset == 9
