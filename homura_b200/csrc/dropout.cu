@@ -14,7 +14,6 @@ namespace hmc {
 namespace {
 
 constexpr int kDropThreads = 256;
-constexpr int kDropDevices = 64;
 constexpr int kPer = 8;     // neighbouring elements a thread takes at a time: two Philox blocks
 template <class C> struct DropRule {
     PhiloxKeys keys;
@@ -227,12 +226,9 @@ HMC_API hmc_status hmc_dropout(hmc_context_t ctx, const hmc_tensor_desc *out, co
                     const T *x = reinterpret_cast<const T *>(layer_base(src)), *r = reinterpret_cast<const T *>(layer_base(residual));
                     if (vectors && same_high) {
                         using G = DropRing<T, RES>;
-                        static bool raised[kDropDevices] = {};  // (a race between threads only repeats the call)
-                        if (G::kBytes > 32768 && (ctx->device >= kDropDevices || !raised[ctx->device])) {
-                            HMC_CUDA(cudaFuncSetAttribute(dropout_flat_kernel<T, RES, RNG>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kBytes),
-                                     "shared memory size of the dropout kernel");
-                            if (ctx->device < kDropDevices) raised[ctx->device] = true;
-                        }
+                        static SharedKnown known;
+                        const hmc_status allowed = allow_shared(ctx, dropout_flat_kernel<T, RES, RNG>, known, G::kBytes, "shared memory size of the dropout kernel");
+                        if (allowed != HMC_OK) return allowed;
                         const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (sizeof(T) == 8 ? 2 : 4);
                         const unsigned flat_grid = static_cast<unsigned>(blocks < resident ? blocks : resident);
                         dropout_flat_kernel<T, RES, RNG><<<flat_grid, kDropThreads, G::kBytes, ctx->stream>>>(o, x, r, n, rule);

@@ -154,11 +154,11 @@ hmc_status launch_resident_forward(hmc_context_t ctx, int dtype, int32_t activat
             const int64_t units = a.samples * a.r.t.tiles;
             const int64_t most = (int64_t{1} << 30) / a.r.cluster;
             if (a.r.t.v == kVector<T>) {
-                static bool raised[kRowDevices] = {};
-                return launch_resident(ctx, resident_kernel<T, kVector<T>, decltype(act)::value>, raised, units < most ? units : most, a.r, a, "group norm kernel launch");
+                static SharedKnown known;
+                return launch_resident(ctx, resident_kernel<T, kVector<T>, decltype(act)::value>, known, units < most ? units : most, a.r, a, "group norm kernel launch");
             }
-            static bool raised[kRowDevices] = {};
-            return launch_resident(ctx, resident_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, raised, units < most ? units : most, a.r, a, "group norm kernel launch");
+            static SharedKnown known;
+            return launch_resident(ctx, resident_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, known, units < most ? units : most, a.r, a, "group norm kernel launch");
         });
     });
 }

@@ -199,12 +199,10 @@ __device__ __forceinline__ Two<double> gather(const Memory &m, const Resident &r
 }
 
 template <class Kernel, class Args>
-hmc_status launch_resident(hmc_context_t ctx, Kernel kernel, bool (&raised)[kRowDevices], int64_t clusters, const Resident &r, const Args &args,
+hmc_status launch_resident(hmc_context_t ctx, Kernel kernel, SharedKnown &known, int64_t clusters, const Resident &r, const Args &args,
                            const char *what) {
-    if (ctx->device >= kRowDevices || !raised[ctx->device]) {
-        HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kResidentShared), what);
-        if (ctx->device < kRowDevices) raised[ctx->device] = true;
-    }
+    const hmc_status s = allow_shared(ctx, kernel, known, kResidentShared, what);
+    if (s != HMC_OK) return s;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(clusters * r.cluster));
     config.blockDim = dim3(kBlock);

@@ -169,11 +169,11 @@ hmc_status launch_resident_backward(hmc_context_t ctx, int dtype, int32_t activa
         using T = decltype(tag);
         return dispatch_activation(activation, [&](auto act) -> hmc_status {
             if (a.r.t.v == kVector<T>) {
-                static bool raised[kRowDevices] = {};
-                return launch_resident(ctx, resident_backward_kernel<T, kVector<T>, decltype(act)::value>, raised, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
+                static SharedKnown known;
+                return launch_resident(ctx, resident_backward_kernel<T, kVector<T>, decltype(act)::value>, known, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
             }
-            static bool raised[kRowDevices] = {};
-            return launch_resident(ctx, resident_backward_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, raised, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
+            static SharedKnown known;
+            return launch_resident(ctx, resident_backward_kernel<T, narrow_vector(sizeof(T)), decltype(act)::value>, known, a.columns * a.r.t.tiles, a.r, a, "group norm gradient kernel launch");
         });
     });
 }

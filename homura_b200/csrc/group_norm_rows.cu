@@ -147,9 +147,9 @@ hmc_status launch_rows_forward(hmc_context_t ctx, int dtype, int32_t activation,
                 const int64_t y = rounds < wanted ? rounds : wanted;
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(y < 65535 ? y : 65535));
                 constexpr int kShared = RowRing<T, V, samples_at_a_time(K) * K>::kBytes;
-                static bool raised[kRowDevices] = {};
+                static SharedKnown known;
                 const auto kernel = rows_kernel<T, V, K, WIDE, decltype(act)::value>;
-                const hmc_status s = raise_shared(ctx, kernel, raised, kShared);
+                const hmc_status s = allow_shared(ctx, kernel, known, kShared, "shared memory size of a group norm kernel");
                 if (s != HMC_OK) return s;
                 kernel<<<grid, kBlock, kShared, ctx->stream>>>(a);
                 return launch_status("group norm kernel launch");

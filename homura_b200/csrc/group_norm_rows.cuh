@@ -185,18 +185,6 @@ template <class T, int V, int WORDS> struct RowRing {
     }
 };
 
-constexpr int kRowDevices = 64;
-// `raised` remembers, per kernel and device, that the kernel may use its dynamic shared memory (with the static part it
-// may pass 48 KB; a race
-// between threads only repeats the call).
-template <class Kernel> inline hmc_status raise_shared(hmc_context_t ctx, Kernel kernel, bool (&raised)[kRowDevices], int bytes) {
-    if (bytes > 32768 && (ctx->device >= kRowDevices || !raised[ctx->device])) {
-        HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory size of a group norm kernel");
-        if (ctx->device < kRowDevices) raised[ctx->device] = true;
-    }
-    return HMC_OK;
-}
-
 struct RowsForwardArgs {
     char *out;
     const char *src;

@@ -143,9 +143,9 @@ hmc_status launch_rows_backward(hmc_context_t ctx, int dtype, int32_t activation
             return dispatch_activation(activation, [&](auto act) -> hmc_status {
                 const dim3 grid(static_cast<unsigned>(a.t.tiles), static_cast<unsigned>(row_blocks));
                 constexpr int kShared = RowRing<T, V, 2 * K>::kBytes;
-                static bool raised[kRowDevices] = {};
+                static SharedKnown known;
                 const auto kernel = rows_backward_kernel<T, V, K, WIDE, decltype(act)::value>;
-                const hmc_status s = raise_shared(ctx, kernel, raised, kShared);
+                const hmc_status s = allow_shared(ctx, kernel, known, kShared, "shared memory size of a group norm kernel");
                 if (s != HMC_OK) return s;
                 kernel<<<grid, kBlock, kShared, ctx->stream>>>(a);
                 return launch_status("group norm gradient kernel launch");

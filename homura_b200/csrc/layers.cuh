@@ -2,6 +2,7 @@
 // three dimensions is walked.
 #pragma once
 
+#include <atomic>
 #include <string>
 
 #include "../../include/homura_cuda_layers.h"
@@ -72,6 +73,22 @@ inline bool layer_vectors(const hmc_tensor_desc *d, int bytes) {
         if (d->sizes[k] > 1 && d->strides[k] * es % bytes != 0) return false;
     }
     return true;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once a device; `known` belongs to the kernel. (Static and dynamic
+// parts together need no asking up to 48 KB; no kernel here has 32 KB of the former. Threads that come at the same time repeat
+// the call.)
+struct SharedKnown {
+    static constexpr int kDevices = 64;
+    std::atomic<bool> allowed[kDevices] = {};
+};
+template <class Kernel> inline hmc_status allow_shared(hmc_context_t ctx, Kernel kernel, SharedKnown &known, int bytes, const char *what) {
+    if (bytes <= 16384) return HMC_OK;
+    const bool kept = ctx->device < SharedKnown::kDevices;
+    if (kept && known.allowed[ctx->device].load(std::memory_order_relaxed)) return HMC_OK;
+    HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+    if (kept) known.allowed[ctx->device].store(true, std::memory_order_relaxed);
+    return HMC_OK;
 }
 
 }  // namespace hmc

@@ -175,8 +175,8 @@ hmc_status launch_forward(hmc_context_t ctx, ForwardArgs &a, int64_t batch, int3
     a.warps_time = shape.warps_time;
     constexpr int kShared = COPY > 0 ? kWarps * kStages * 2 * R * Ring<T, V, COPY>::kRow : 0;
     const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
-        static bool raised[kKnownDevices] = {};
-        return launch(ctx, forward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, raised, kShared, shape, a,
+        static SharedKnown known;
+        return launch(ctx, forward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, known, kShared, shape, a,
                       "linear recurrence kernel launch");
     };
     return dispatch_flags(flags, go);

@@ -305,17 +305,11 @@ template <class F> hmc_status dispatch_flags(int32_t flags, F &&f) {
     }
 }
 
-constexpr int kKnownDevices = 64;
-
-// `raised` remembers, per kernel and device, that the kernel may use its dynamic shared memory (a race between threads
-// only repeats the call).
 template <class Kernel, class Args>
-hmc_status launch(hmc_context_t ctx, Kernel kernel, bool (&raised)[kKnownDevices], int shared, const Shape &shape, const Args &args,
+hmc_status launch(hmc_context_t ctx, Kernel kernel, SharedKnown &known, int shared, const Shape &shape, const Args &args,
                   const char *what) {
-    if (shared > 0 && (ctx->device >= kKnownDevices || !raised[ctx->device])) {
-        HMC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared), what);
-        if (ctx->device < kKnownDevices) raised[ctx->device] = true;
-    }
+    const hmc_status s = allow_shared(ctx, kernel, known, shared, what);
+    if (s != HMC_OK) return s;
     cudaLaunchConfig_t config{};
     config.dynamicSmemBytes = static_cast<size_t>(shared);
     config.gridDim = dim3(shape.grid);

@@ -203,9 +203,9 @@ hmc_status launch_backward(hmc_context_t ctx, BackwardArgs &a, int64_t batch, in
     const Shape shape = plan_launch(batch, a.time, a.channels, flat, V, R, kPerSm<T>, &a.columns);
     a.warps_time = shape.warps_time;
     const auto go = [&](auto sigmoid, auto complement) -> hmc_status {
-        static bool raised[kKnownDevices] = {};
+        static SharedKnown known;
         constexpr int kShared = COPY > 0 ? kWarps * kStages * kStageRows<R, decltype(complement)::value> * Ring<T, V, COPY>::kRow : 0;
-        return launch(ctx, backward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, raised, kShared, shape, a,
+        return launch(ctx, backward_kernel<T, V, R, COPY, decltype(sigmoid)::value, decltype(complement)::value>, known, kShared, shape, a,
                       "linear recurrence gradient kernel launch");
     };
     return dispatch_flags(flags, go);

@@ -1,10 +1,12 @@
 """Where the trainable operators of include/homura_cuda_layers.h could go wrong by more than rounding: groups of one value, signs
 at an activation's kink, long sums, logits and values at the ends of their types. Expected values are exact or follow from
 the definition; a tolerance counts the roundings on a value's way."""
+import threading
+
 import numpy as np
 import pytest
 
-from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS, BackendError, CudaBackend
+from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS, BackendError, CudaBackend, Generator
 from layers_reference import raw, value
 
 pytestmark = pytest.mark.gpu
@@ -212,3 +214,39 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable(dtype):
                 assert (a == v).all()
     finally:
         be.close()
+
+
+def test_threads_that_call_for_the_first_time_at_once(cuda):
+    """Eight threads with a context each: kernels that need more shared memory than a launch gets unasked."""
+    rng = np.random.default_rng(4)
+    x, gate = rng.normal(size=(2, 700, 72)), rng.normal(size=(2, 700, 72))
+    ready, results = threading.Barrier(8), [None] * 8
+
+    def work(k):
+        be = CudaBackend(0)
+        try:
+            found = []
+            ready.wait(60)
+            for dtype in (BF16, F16, F32, F64):
+                up = lambda v: be.upload(raw(v, dtype), dtype)
+                h, y, z = (be.empty(x.shape, dtype) for _ in range(3))
+                stats = [be.empty((2, 6), stat_dtype(dtype)) for _ in range(2)]
+                be.linear_recurrence(h, up(gate), up(x), sigmoid=True)
+                be.group_norm(y, h, 6, None, None, *stats, activation="silu")
+                be.dropout(z, y, Generator(3), 0.25, residual=h)
+                grads = [be.empty(x.shape, dtype) for _ in range(3)]
+                be.group_norm_backward(grads[0], h, z, *stats, 6, activation="silu")
+                be.linear_recurrence_backward(grads[1], grads[2], up(gate), None, h, grads[0], sigmoid=True)
+                found += [be.download(v) for v in (h, y, z, *grads)]
+            results[k] = found
+        finally:
+            be.close()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert all(r is not None for r in results)
+    for r in results[1:]:
+        assert all((a.view(np.uint8) == v.view(np.uint8)).all() for a, v in zip(results[0], r))
