@@ -1,13 +1,15 @@
 """Where the trainable operators of include/homura_cuda_layers.h could go wrong by more than rounding: groups of one value, signs
 at an activation's kink, long sums, logits and values at the ends of their types. Expected values are exact or follow from
 the definition; a tolerance counts the roundings on a value's way."""
+import math
 import threading
 
 import numpy as np
 import pytest
 
 from homura_b200.host import BF16, DTYPE_NAMES, F16, F32, F64, FLOATS, BackendError, CudaBackend, Generator
-from layers_reference import raw, value
+from layers_reference import dropout, group_norm, group_norm_backward, raw, rounded, value, within
+from test_gpu_recurrence import check_backward, check_forward
 
 pytestmark = pytest.mark.gpu
 
@@ -182,6 +184,30 @@ def test_products_of_gates_beyond_the_range_show(cuda):
                 assert (right | ((start != 0.0) & ~np.isfinite(got))).all(), (t, start, got[~right][:4])
 
 
+@pytest.mark.parametrize("dtype,size,kind", [(F32, (1300003, 1, 8, 1), "silu"), (BF16, (200001, 1, 64, 1), "gelu"), (F16, (30011, 3, 8, 2), None),
+                                             (F64, (20011, 1, 12, 3), "relu"), (BF16, (3001, 20, 16, 2), "silu")], ids=str)
+def test_many_samples(cuda, dtype, size, kind):
+    """Hundreds of row blocks, runs of more than eight samples a team, and their partials for dweight and dbias."""
+    n, s, c, groups = size
+    rng = np.random.default_rng(n)
+    sd = stat_dtype(dtype)
+    x, d = raw(rng.normal(size=(n, s, c)), dtype), raw(rng.normal(0.3, 1, size=(n, s, c)), dtype)
+    w, b = raw(rng.normal(1, 0.3, c), sd), raw(rng.normal(0, 0.3, c), sd)
+    forward = group_norm(value(x, dtype), value(w, sd), value(b, sd), groups, 1e-5, kind, dtype)
+    y, mean, rstd = norm(cuda, x, dtype, groups, w, b, kind)
+    within(value(y, dtype), forward[0], rounded(forward[1], forward[0], dtype), "out")
+    within(mean, forward[2], rounded(forward[3], forward[2], sd), "mean")
+    within(rstd, forward[4], rounded(forward[5], forward[4], sd), "rstd")
+    up = lambda v, dt: cuda.upload(v, dt)
+    dx, dw, db = cuda.empty(x.shape, dtype), cuda.empty((c,), sd), cuda.empty((c,), sd)
+    cuda.group_norm_backward(dx, up(x, dtype), up(d, dtype), up(mean, sd), up(rstd, sd), groups, up(w, sd), up(b, sd), dw, db, activation=kind)
+    want = group_norm_backward(value(x, dtype), value(d, dtype), mean.astype(np.float64), rstd.astype(np.float64), value(w, sd), value(b, sd),
+                               groups, kind, dtype)
+    within(value(cuda.download(dx), dtype), want[0], rounded(want[1], want[0], dtype), "dsrc")
+    within(cuda.download(dw), want[2], rounded(want[3], want[2], sd), "dweight")
+    within(cuda.download(db), want[4], rounded(want[5], want[4], sd), "dbias")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32, F64], ids=["bf16", "f32", "f64"])
 def test_a_wait_that_runs_out_is_reported_and_leaves_the_context_usable(dtype):
     """The blocks of a cluster wait for one another's sums with a limit. With a limit of 0 all give up at once, every peer alive: the
@@ -250,3 +276,51 @@ def test_threads_that_call_for_the_first_time_at_once(cuda):
     assert all(r is not None for r in results)
     for r in results[1:]:
         assert all((a.view(np.uint8) == v.view(np.uint8)).all() for a, v in zip(results[0], r))
+
+
+@pytest.mark.parametrize("dtype", [F32, F64], ids=["f32", "f64"])
+@pytest.mark.parametrize("s", [1, 200, 40000])
+def test_activations_keep_their_relative_precision_in_the_tails(cuda, dtype, s):
+    """A weight of 0 leaves the bias as the activation's argument. Relative bounds in units of the computation type, with the
+    rounding of the exponential's argument as its leading term: u = 2^-24 (2^-53); ex2.approx 4, rcp.approx 2, the fit of erfc 2
+    and its polynomial 4, sums and products 1 each."""
+    z = np.concatenate([-np.geomspace(1e-6, 13.0, 250), np.geomspace(1e-6, 30.0, 246), [-20.0, -40.0, -80.0, 0.0]])
+    z = raw(z, dtype)
+    c = z.size
+    x = raw(np.where(np.arange(s * c).reshape(1, s, c) % 2, 1.0, -1.0), dtype)
+    u, least = (2.0**-53, 2.0**-1022) if dtype == F64 else (2.0**-24, 2.0**-126)
+    z64 = value(z, dtype)
+    inner = np.sqrt(8 / np.pi) * (z64 + 0.044715 * z64**3)
+    sigmoid = lambda v: np.exp(np.minimum(v, 0)) / (1 + np.exp(-np.abs(v)))
+    # gelu: -z^2 / 2 is rounded in x = |z| / sqrt(2) (twice, squared), in the fused sum and in the product with log2(e) (twice)
+    wants = {"silu": (z64 * sigmoid(z64), 2 * np.abs(z64) + 12),
+             "gelu": (z64 * np.array([0.5 * math.erfc(-v / math.sqrt(2)) for v in z64]), 3 * z64**2 + 20),
+             "gelu_tanh": (z64 * sigmoid(inner), 6 * np.abs(inner) + 14)}
+    for kind, (want, units) in wants.items():
+        got, _, _ = norm(cuda, x, dtype, 4, np.zeros(c), z64, kind)
+        off = np.abs(value(got, dtype)[0] - want)
+        # (results below the smallest normal number, times |z|, are flushed)
+        assert (off <= (units + 1) * u * np.abs(want) + 2 * np.abs(z64) * least).all(), (kind, z64[(off / np.abs(want + least)).argmax()], (off / np.abs(want + least)).max() / u)
+
+
+@pytest.mark.parametrize("layout", ["half", "time first", "time last"])
+@pytest.mark.parametrize("dtype", [F16, F64], ids=["f16", "f64"])
+def test_layouts_of_the_other_types(cuda, dtype, layout):
+    rng = np.random.default_rng(6)
+    for size in ((2, 70, 66), (3, 33, 31), (1, 600, 64)):
+        for reverse in (False, True):
+            check_forward(cuda, rng, size, dtype, True, layout, sigmoid=True, complement=True, reverse=reverse)
+            check_backward(cuda, rng, size, dtype, True, layout, sigmoid=True, complement=True, reverse=reverse)
+
+
+@pytest.mark.parametrize("dtype", [F16, F64], ids=["f16", "f64"])
+def test_dropout_of_strided_operands_in_the_other_types(cuda, dtype):
+    """The mask goes by logical positions; the residual is broadcast along the first dimension."""
+    rng = np.random.default_rng(7)
+    x, r = raw(rng.normal(size=(5, 33, 18)), dtype), raw(rng.normal(size=(1, 33, 18)), dtype)
+    turned = cuda.upload(np.ascontiguousarray(x.transpose(2, 0, 1)), dtype).transpose(0, 1).transpose(1, 2)
+    for p in (0.0, 0.3, 1.0):
+        out, gen = cuda.empty(x.shape, dtype), Generator(11)
+        seed, offset = cuda.dropout(out, turned, gen, p, residual=cuda.upload(r, dtype).expand(5, 33, 18))
+        want, bound, _ = dropout(value(x, dtype), value(r, dtype), p, seed, offset, dtype)
+        within(value(cuda.download(out), dtype), want, rounded(bound, want, dtype), f"p {p}")
