@@ -27,7 +27,9 @@ __device__ __forceinline__ double logistic(double z) { return 1.0 / (1.0 + exp(-
 // x >= 0, the Chebyshev fit of Press, Teukolsky, Vetterling and Flannery (Numerical Recipes, "erfcc"): about twenty operations
 // without a branch, half of erff's. The fit is good to 1.2e-7 of its value everywhere; the roundings of the exponential's
 // argument, which grows as z^2 / 2, add up to 3 z^2 2^-24 for z < 0 (seen: 3e-7 down to z = -1, 9e-7 to -3, 4e-6 to -6, 1e-5 to
-// -13, where z times it is 1e-37), which an absolute error of a unit of z never shows.
+// -13, where z times it is 1e-37), which an absolute error of a unit of z never shows. With erfcf and expf in the place of this and
+// of density's exponential, the gradients of f32 [16384, 1, 4096] with gelu take 240 us instead of 195 and are off by 1.1e-7
+// of their size instead of 1.2e-7: what is left is the f32 arithmetic around them.
 __device__ __forceinline__ float normal_cdf(float z) {
     const float x = fabsf(z) * 0.70710678118654752440f;
     float t;

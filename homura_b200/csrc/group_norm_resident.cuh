@@ -31,7 +31,7 @@ struct Resident {
     int32_t shared;
 };
 
-// Against the pieces merged by a second kernel: f16 [16, 4096, 320] in 32 groups 82 us in pieces, 42 here; f32 [487, 384, 58] in 2
+// Against the pieces merged by a second kernel: f16 [16, 4096, 320] in 32 groups 82 us in pieces, 43 here; f32 [487, 384, 58] in 2
 // groups (by words) 97 and 28. `operands` tensors are kept. Tiles are made wide enough for whole 128-byte lines where the groups allow, and, where
 // there are few positions, as wide as gives a block some tens of KB of work.
 inline Resident make_resident(const Problem &p, int vector, int operands) {

@@ -1,6 +1,6 @@
 // Group norm where a group of one sample fits the registers of a team of lanes: every token by itself (one position), or
 // few positions. One pass: a value is read once and written once (bf16 [32768, 1, 4096] in 32 groups: 1473 us in tiles of rows
-// with a block's sums for every sample, 110 here).
+// with a block's sums for every sample, 107 to 115 here).
 //
 // A team is a power of two of lanes within a warp (or, WIDE, the whole block); a lane keeps K vectors of V neighbouring
 // channels of its team's group, the same channels for every sample it takes, so parameters (and, backward, the sums for

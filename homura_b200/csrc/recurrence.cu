@@ -238,7 +238,7 @@ HMC_API hmc_status hmc_linear_recurrence(hmc_context_t ctx, const hmc_tensor_des
             const bool flat = flat_columns(channels, V), lines = wide && !flat;
             if constexpr (sizeof(T) < 8) {
                 // Sixteen rows a lane halve the exchanges, two blocks an SM then: where that many blocks take all channels (bf16
-                // [8, 2048, 4096]: 112 us with eight rows and four blocks an SM, 85 with sixteen).
+                // [8, 2048, 4096]: 117 us with eight rows and four blocks an SM, 88 with sixteen; f32 [1, 65521, 1000]: 214 and 169).
                 const int64_t warps = flat ? ceil_div(batch * channels, int64_t{32} * V) : batch * ceil_div(channels, int64_t{32} * V);
                 if (warps <= int64_t{148} * 2 * kWarps) {
                     return lines ? launch_forward<T, V, 16, 16>(ctx, a, batch, flags) : launch_forward<T, V, 16, kWord>(ctx, a, batch, flags);

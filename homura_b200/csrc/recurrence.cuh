@@ -228,7 +228,7 @@ struct Shape {
 
 // WT and the cluster grow while every block still finds a place at once, `per_sm` on an SM, and the time axis feeds them:
 // a second, partly filled wave costs more than the warps it brings (the gradients of bf16 [4, 4096, 2048] at two blocks an SM:
-// 110 us with 512 blocks in clusters of four, 94 with 256 in clusters of two). The constant is B200's SM count, not the device's,
+// 101 us with 512 blocks in clusters of four, 94 with 256 in clusters of two). The constant is B200's SM count, not the device's,
 // so that the order of folding is the same everywhere.
 inline Shape plan_launch(int64_t batch, int64_t time, int64_t channels, bool flat, int v, int rows, int per_sm, Columns *columns) {
     *columns = Columns{channels, 0, 0, channels / v, batch * (channels / v), flat ? 1 : 0};
