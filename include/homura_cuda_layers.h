@@ -66,9 +66,9 @@ hmc_status hmc_linear_recurrence_backward(hmc_context_t ctx, const hmc_tensor_de
  * the view src. weight and bias (both or neither) are [channels] of T or of F32, alike. mean and rstd (both or neither)
  * receive the groups' moments, [samples, groups] of F32 (F64 when T is F64), for the backward pass. The moments are
  * taken in two passes over values held on chip: first the mean, then the deviations from it. Where a group is cut into
- * pieces, those are merged pairwise in f64 or, for F16, BF16 and F32 pieces in shared memory, through f64 sums of
- * n mean and n mean^2, which lose 2^-52 (mean / deviation)^2 of the variance, a sixteenth of what the rounding of a piece's f32
- * mean does to it. A constant group becomes its bias as long as the sums of its elements are numbers of the computation
+ * pieces, those are merged in f64, pairwise or (F16, BF16 and F32 in shared memory) through sums of n mean and n mean^2. A
+ * piece's mean is rounded to the computation type before that, which does to the moments no more than rounding every element
+ * once more would (2^-23 |mean| / deviation of the variance). A constant group becomes its bias as long as the sums of its elements are numbers of the computation
  * type. A NaN or an infinity makes its own group NaN, no other. The workspace has hmc_group_norm_workspace bytes
  * (0: NULL is fine), 16-byte aligned. */
 hmc_status hmc_group_norm_workspace(const hmc_tensor_desc *src, int32_t groups, int32_t backward, int64_t *bytes);
