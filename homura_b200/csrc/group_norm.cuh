@@ -59,6 +59,14 @@ template <class C> __device__ __forceinline__ C gelu_inner(C z, C &slope) {
     return k * z * (C(1) + q);
 }
 
+// z between -64 and 64, a NaN passed on.
+__device__ __forceinline__ float within_64(float z) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(-64.0f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(z) : "f"(64.0f));
+    return z;
+}
+__device__ __forceinline__ double within_64(double z) { return z > 64.0 ? 64.0 : (z < -64.0 ? -64.0 : z); }
+
 // xhat * w + b: in two roundings before relu, whose derivative goes by the sign alone, so that the sign is that of the
 // plain formula; fused otherwise. Every forward and backward kernel takes the same steps from x on, (x - mean) * rstd first,
 // so that all find the same z: moments and parameters are not folded into one product and sum, which leaves
@@ -87,8 +95,7 @@ template <int ACT, class C> __device__ __forceinline__ C through(C d, C z) {
     } else if constexpr (ACT == HMC_UNARY_GELU_TANH) {
         // (beyond 64 s is 0 or 1 to the last bit, but the inner slope and its product with z overflow in the end: held there)
         C slope;
-        const C s = logistic(gelu_inner(z, slope)), held = z > C(64) ? C(64) : (z < C(-64) ? C(-64) : z);
-        gelu_inner(held, slope);
+        const C held = within_64(z), s = logistic(gelu_inner(held, slope));
         return d * (s * m_fma(held * (C(1) - s), slope, C(1)));
     } else return d;
 }

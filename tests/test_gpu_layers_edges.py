@@ -97,6 +97,13 @@ def test_sums_over_long_runs_of_rows(cuda):
         assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
 
 
+def test_sums_over_long_runs_of_whole_vectors(cuda):
+    """The same with 16-byte vectors, whose runs are shorter instead: 15 rows at a time, 267 a thread."""
+    dw, db, want = one_large_many_small(cuda, list(range(15)), 4000, 136, 600, F16, 1)
+    for got in (dw, db):
+        assert (np.abs(got - want) <= (65 * 2.0**-24 + 2.0**-24) * want).all(), (got, want)
+
+
 def test_sums_over_a_clusters_rows(cuda):
     """Words in a cluster's shared memory, 98 rows a thread, the first of each thread large."""
     rows = [r for r in range(6272) if r % 784 < 8]
