@@ -39,6 +39,8 @@ template <class C> struct alignas(2 * sizeof(C)) Step {
 
 // A step applied to the value before it. A product of gates may have overflowed: a state of zero stays zero all the same, any
 // other becomes infinite or no number, never a finite wrong one. (A NaN or infinite gate shows in b, which is folded from zero.)
+// The selection lengthens the chain of folds that a lane waits for: f32 [1, 65536, 8], all of it exchanges, 106 us with products held
+// at the largest number instead, 112 with it; bf16 [8, 2048, 4096] 86 and 87.
 template <class C> __device__ __forceinline__ C fold(Step<C> s, C v) { return v == C(0) ? s.b : m_fma(s.a, v, s.b); }
 
 // Rows and channels of one operand, in elements; t may be negative.
